@@ -17,6 +17,7 @@
 constexpr int MAX_DEVICES_POOL = 16;
 
 #include "../../include/gnnx.h"
+#include "gnnx_error.hpp"
 #include "gnnx_kernels.hpp"
 #include "gnnx_resident.hpp"
 #include "gnnx_sparse.hpp"
@@ -29,6 +30,13 @@ using namespace gnnx;
 static thread_local std::string g_err;
 static int fail(const std::string& m) {
     g_err = m;
+    return 1;
+}
+int gnnx::set_error(const char* text) noexcept {
+    try {
+        g_err = text;
+    } catch (...) {      // out of memory: the text before stays
+    }
     return 1;
 }
 #define HIPCK(x)                                                                                   \

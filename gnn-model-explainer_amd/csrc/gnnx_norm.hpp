@@ -1,0 +1,212 @@
+// gnnx_norm.hpp — layer norm (ReLU before it, gain / offset, their gradients), dropout from a counter-based generator, and the two in one
+// pass: the run between two graph convolutions of an encoder (models.py:230-267: ReLU, norm; :58-61: the next layer's dropout).
+//
+// x is a matrix of `rows` rows and `cols` columns, the elements of a row contiguous, the rows x_stride elements apart; v = max(x, 0) or x.
+//   forward    mu = mean v, var = mean (v - mu)^2, rstd = (var + eps)^-1/2, xhat = (v - mu) rstd, y = xhat w + b, d = dropout(y)
+//   backward   dy = dL/dy + dropout(dL/dd), g = dy w, c1 = mean g, c2 = mean g xhat, dx = rstd (g - c1 - xhat c2) [x > 0],
+//              dw = sum over rows of dy xhat, db = sum over rows of dy
+//   dropout    word(r, c) = word c mod 4 of Philox-4x32-10 at counter (c / 4, r mod 2^32, r / 2^32, step) under the key `seed`; the element stays,
+//              scaled by 1 / (1 - p), where word >= round(p 2^32), and is 0 otherwise.  Recomputed wherever it is needed, never stored.
+// All arithmetic in fp32 whatever the storage type (fp32, bf16, fp16); one rounding, at the store.
+#pragma once
+#include <stdint.h>
+
+namespace gnnx {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+struct DropArgs {
+    int32_t on;              // 0: nothing is dropped (threshold 0)
+    uint32_t last_dropped;   // threshold - 1: a word is dropped where word <= last_dropped
+    float scale;
+    uint32_t k0, k1, step;
+    const int64_t* state;    // device (seed, step) or null: read when the kernel runs; `step` is added to it
+    int64_t row0;            // the row of the whole tensor that row 0 here is
+};
+
+struct NormArgs {
+    int64_t rows, cols, x_stride, dy_stride, dd_stride;
+    const void *x, *w, *b, *dy, *dd;
+    void *y, *d, *dx, *dw, *db;
+    float *mean, *rstd;
+    float eps, relu_floor;   // v = x < relu_floor ? relu_floor : x (0, or -inf without ReLU; NaN stays NaN)
+    int32_t relu;
+    int32_t w_is_f32;        // type of w, b, dw, db: 1 fp32, 0 the type of x
+    float* part;             // [parts][2][cols] partial column sums of the backward pass
+    int32_t parts;
+    DropArgs drop;
+};
+
+struct Philox4 { uint32_t w[4]; };
+
+// Philox-4x32-10: Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011 (the constants are the paper's).
+__device__ __forceinline__ Philox4 philox(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1) {
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {
+        const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
+        c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+        c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+        c1 = (uint32_t)p1;
+        c3 = (uint32_t)p0;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    return {{c0, c1, c2, c3}};
+}
+
+struct DropKey { uint32_t k0, k1, step; };
+__device__ __forceinline__ DropKey drop_key(const DropArgs& a) {
+    if (!a.state) return {a.k0, a.k1, a.step};
+    const uint64_t seed = (uint64_t)a.state[0];
+    return {(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)((uint64_t)a.state[1] + a.step)};
+}
+// the four words of columns 4 block .. 4 block + 3 of row r
+__device__ __forceinline__ Philox4 drop_words(const DropArgs& a, const DropKey& k, int64_t r, uint32_t block) {
+    const uint64_t row = (uint64_t)(r + a.row0);
+    return philox(block, (uint32_t)row, (uint32_t)(row >> 32), k.step, k.k0, k.k1);
+}
+__device__ __forceinline__ float dropped(const DropArgs& a, uint32_t word, float v) {
+    return word > a.last_dropped || !a.on ? v * a.scale : 0.0f;
+}
+
+__device__ __forceinline__ float wave_total(float v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+template <class T>
+__device__ __forceinline__ float param_at(const void* p, int32_t is_f32, int64_t c) {
+    return is_f32 ? static_cast<const float*>(p)[c] : (float)static_cast<const T*>(p)[c];
+}
+
+// One wave per row, the row read again for each of the three passes (mean, squared distance from it, output).
+template <class T, bool DROP>
+__global__ __launch_bounds__(256) void k_norm_forward(NormArgs a) {
+    const int lane = threadIdx.x & 63;
+    const float inv = 1.0f / (float)a.cols;
+    const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * 4) {
+        const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
+        float s = 0.0f;
+        for (int64_t c = lane; c < a.cols; c += 64) {
+            const float v = (float)x[c];
+            s += v < a.relu_floor ? a.relu_floor : v;
+        }
+        const float mean = wave_total(s) * inv;
+        s = 0.0f;
+        for (int64_t c = lane; c < a.cols; c += 64) {
+            float v = (float)x[c];
+            v = (v < a.relu_floor ? a.relu_floor : v) - mean;
+            s += v * v;
+        }
+        const float rstd = 1.0f / sqrtf(wave_total(s) * inv + a.eps);
+        if (lane == 0 && a.mean) {
+            a.mean[r] = mean;
+            a.rstd[r] = rstd;
+        }
+        for (int64_t c = lane; c < a.cols; c += 64) {
+            float v = (float)x[c];
+            v = ((v < a.relu_floor ? a.relu_floor : v) - mean) * rstd;
+            if (a.w) v *= param_at<T>(a.w, a.w_is_f32, c);
+            if (a.b) v += param_at<T>(a.b, a.w_is_f32, c);
+            if (a.y) static_cast<T*>(a.y)[r * a.cols + c] = (T)v;
+            if (DROP) static_cast<T*>(a.d)[r * a.cols + c] = (T)dropped(a.drop, drop_words(a.drop, key, r, (uint32_t)(c >> 2)).w[c & 3], v);
+        }
+    }
+}
+
+// dL/dy at (r, c): the gradient of the kept output plus that of the dropped one
+template <class T, bool DROP>
+__device__ __forceinline__ float norm_dy(const NormArgs& a, const DropKey& key, int64_t r, int64_t c) {
+    float g = a.dy ? (float)static_cast<const T*>(a.dy)[r * a.dy_stride + c] : 0.0f;
+    if (DROP) g += dropped(a.drop, drop_words(a.drop, key, r, (uint32_t)(c >> 2)).w[c & 3], (float)static_cast<const T*>(a.dd)[r * a.dd_stride + c]);
+    return g;
+}
+
+template <class T, bool DROP>
+__global__ __launch_bounds__(256) void k_norm_backward_rows(NormArgs a) {
+    const int lane = threadIdx.x & 63;
+    const float inv = 1.0f / (float)a.cols;
+    const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * 4) {
+        const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        float s1 = 0.0f, s2 = 0.0f;
+        for (int64_t c = lane; c < a.cols; c += 64) {
+            float v = (float)x[c], g = norm_dy<T, DROP>(a, key, r, c);
+            v = ((v < a.relu_floor ? a.relu_floor : v) - mean) * rstd;
+            if (a.w) g *= param_at<T>(a.w, a.w_is_f32, c);
+            s1 += g;
+            s2 += g * v;
+        }
+        const float c1 = wave_total(s1) * inv, c2 = wave_total(s2) * inv;
+        for (int64_t c = lane; c < a.cols; c += 64) {
+            const float xv = (float)x[c];
+            float v = xv, g = norm_dy<T, DROP>(a, key, r, c);
+            v = ((v < a.relu_floor ? a.relu_floor : v) - mean) * rstd;
+            if (a.w) g *= param_at<T>(a.w, a.w_is_f32, c);
+            g = rstd * (g - c1 - v * c2);
+            static_cast<T*>(a.dx)[r * a.cols + c] = (T)(a.relu && xv <= 0.0f ? 0.0f : g);
+        }
+    }
+}
+
+// Partial column sums: workgroup (column tile of 64, part) adds the rows r = 4 part + wave mod 4 parts; the four waves join in LDS.
+template <class T, bool DROP>
+__global__ __launch_bounds__(256) void k_norm_backward_cols(NormArgs a) {
+    __shared__ float sums[2][4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t tiles = (a.cols + 63) / 64;
+    const int64_t part = blockIdx.x / tiles, c = (blockIdx.x % tiles) * 64 + lane;
+    const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
+    float sw = 0.0f, sb = 0.0f;
+    if (c < a.cols)
+        for (int64_t r = part * 4 + wave; r < a.rows; r += (int64_t)a.parts * 4) {
+            float v = (float)(static_cast<const T*>(a.x)[r * a.x_stride + c]);
+            const float g = norm_dy<T, DROP>(a, key, r, c);
+            v = ((v < a.relu_floor ? a.relu_floor : v) - a.mean[r]) * a.rstd[r];
+            sw += g * v;
+            sb += g;
+        }
+    sums[0][wave][lane] = sw;
+    sums[1][wave][lane] = sb;
+    __syncthreads();
+    if (wave < 2 && c < a.cols) a.part[(part * 2 + wave) * a.cols + c] = (sums[wave][0][lane] + sums[wave][1][lane]) + (sums[wave][2][lane] + sums[wave][3][lane]);
+}
+
+// The partial sums of a column, in part order.
+template <class T>
+__global__ __launch_bounds__(256) void k_norm_join(NormArgs a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;      // dw's columns, then db's
+    if (i >= 2 * a.cols) return;
+    const bool is_b = i >= a.cols;
+    const int64_t c = is_b ? i - a.cols : i;
+    void* out = is_b ? a.db : a.dw;
+    if (!out) return;
+    float s = 0.0f;
+    for (int p = 0; p < a.parts; ++p) s += a.part[((int64_t)p * 2 + is_b) * a.cols + c];
+    if (a.w_is_f32) static_cast<float*>(out)[c] = s;
+    else static_cast<T*>(out)[c] = (T)s;
+}
+
+// One thread per four columns of a row.
+template <class T>
+__global__ __launch_bounds__(256) void k_dropout(int64_t rows, int64_t cols, int64_t stride, const T* x, T* y, DropArgs d) {
+    const DropKey key = drop_key(d);
+    const int64_t blocks = (cols + 3) / 4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * blocks; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / blocks, k = i % blocks;
+        Philox4 q = {};
+        if (d.on) q = drop_words(d, key, r, (uint32_t)k);
+        for (int j = 0; j < 4; ++j) {
+            const int64_t c = 4 * k + j;
+            if (c >= cols) break;
+            const float v = (float)x[r * stride + c];
+            y[r * cols + c] = (T)dropped(d, q.w[j], v);
+        }
+    }
+}
+
+}  // namespace gnnx

@@ -1,0 +1,156 @@
+// gnnx_ops.hip — C ABI (include/gnnx.h) over the encoder-layer operators of gnnx_norm.hpp: layer norm, dropout, and both in one pass.
+// Host side only: argument checks, launch shapes.  The library keeps nothing between calls; workspaces are the caller's.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdio>
+#include <limits>
+
+#include "../../include/gnnx.h"
+#include "gnnx_error.hpp"
+#include "gnnx_norm.hpp"
+
+using namespace gnnx;
+
+namespace {
+
+int launched(const char* what) {
+    const hipError_t e = hipGetLastError();
+    if (e == hipSuccess) return 0;
+    char text[256];
+    snprintf(text, sizeof(text), "%s: %s", what, hipGetErrorString(e));
+    return set_error(text);
+}
+
+// workgroups of a launch that walks `items` with a grid stride: at most 2^22 (256 threads each: the 32-bit work-item limit of a launch)
+unsigned grid_of(int64_t items, int64_t per_group) {
+    const int64_t g = (items + per_group - 1) / per_group;
+    return (unsigned)(g < 1 ? 1 : g > (int64_t(1) << 22) ? (int64_t(1) << 22) : g);
+}
+
+const char* drop_args(const gnnx_drop* d, DropArgs* out) {
+    *out = DropArgs{};
+    if (!d) return nullptr;
+    if (!(d->p >= 0.0 && d->p <= 1.0)) return "dropout: p must be in [0, 1]";
+    const double thr = std::nearbyint(d->p * 4294967296.0);       // 0 .. 2^32, ties to even (Python's round)
+    out->on = thr > 0.0;
+    out->last_dropped = out->on ? (uint32_t)(thr - 1.0) : 0u;
+    out->scale = d->p < 1.0 ? (float)(1.0 / (1.0 - d->p)) : 0.0f;
+    out->k0 = (uint32_t)d->seed;
+    out->k1 = (uint32_t)(d->seed >> 32);
+    out->step = d->step;
+    out->state = d->state;
+    out->row0 = d->row_offset;
+    return nullptr;
+}
+
+const char* norm_args(const gnnx_norm* n, NormArgs* a) {
+    if (!n) return "null argument";
+    if (n->type < 0 || n->type > 2) return "layer norm: type must be 0 (fp32), 1 (bf16) or 2 (fp16)";
+    if (n->rows < 0 || n->cols < 1 || n->cols >= (int64_t(1) << 30)) return "layer norm: needs rows >= 0 and 1 <= cols < 2^30";
+    if (n->x_stride < 0 || n->dy_stride < 0 || n->dd_stride < 0) return "layer norm: row strides must not be negative";
+    if (!(n->eps >= 0.0f)) return "layer norm: eps must not be negative";
+    *a = NormArgs{};
+    a->rows = n->rows;
+    a->cols = n->cols;
+    a->x_stride = n->x_stride;
+    a->dy_stride = n->dy_stride;
+    a->dd_stride = n->dd_stride;
+    a->x = n->x;
+    a->w = n->w;
+    a->b = n->b;
+    a->dy = n->dy;
+    a->dd = n->dd;
+    a->y = n->y;
+    a->d = n->d;
+    a->dx = n->dx;
+    a->dw = n->dw;
+    a->db = n->db;
+    a->mean = n->mean;
+    a->rstd = n->rstd;
+    a->eps = n->eps;
+    a->relu = n->relu != 0;
+    a->relu_floor = n->relu ? 0.0f : -std::numeric_limits<float>::infinity();
+    a->w_is_f32 = n->w_is_f32 != 0 || n->type == GNNX_F32;
+    return nullptr;
+}
+
+int col_parts(int64_t rows, int64_t cols) {
+    const int64_t tiles = (cols + 63) / 64;
+    int64_t parts = 2048 / tiles;
+    if (parts > (rows + 15) / 16) parts = (rows + 15) / 16;
+    return (int)(parts < 1 ? 1 : parts);
+}
+
+template <class T>
+void run_forward(const NormArgs& a, hipStream_t s) {
+    if (a.d) hipLaunchKernelGGL((k_norm_forward<T, true>), dim3(grid_of(a.rows, 4)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_norm_forward<T, false>), dim3(grid_of(a.rows, 4)), dim3(256), 0, s, a);
+}
+
+template <class T, bool DROP>
+void run_backward(const NormArgs& a, hipStream_t s) {
+    if (a.dx && a.rows) hipLaunchKernelGGL((k_norm_backward_rows<T, DROP>), dim3(grid_of(a.rows, 4)), dim3(256), 0, s, a);
+    if (!a.dw && !a.db) return;
+    const unsigned tiles = (unsigned)((a.cols + 63) / 64);
+    hipLaunchKernelGGL((k_norm_backward_cols<T, DROP>), dim3(tiles * (unsigned)a.parts), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_norm_join<T>), dim3((unsigned)((2 * a.cols + 255) / 256)), dim3(256), 0, s, a);
+}
+
+}  // namespace
+
+extern "C" int gnnx_layer_norm_forward(const gnnx_norm* n, const gnnx_drop* drop, void* stream) {
+    NormArgs a;
+    if (const char* e = norm_args(n, &a)) return set_error(e);
+    if (const char* e = drop_args(drop, &a.drop)) return set_error(e);
+    if (a.rows == 0) return 0;
+    if (!a.y && !a.d) return set_error("layer norm: no output");
+    if ((a.d != nullptr) != (drop != nullptr)) return set_error("layer norm: a dropped output and its dropout go together");
+    if ((a.mean != nullptr) != (a.rstd != nullptr)) return set_error("layer norm: mean and rstd go together");
+    if (!a.x) return set_error("null argument");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (n->type == GNNX_F32) run_forward<float>(a, s);
+    else if (n->type == GNNX_BF16) run_forward<bf16_t>(a, s);
+    else run_forward<f16_t>(a, s);
+    return launched("gnnx_layer_norm_forward");
+}
+
+extern "C" size_t gnnx_layer_norm_workspace_bytes(int32_t, int64_t rows, int64_t cols) {
+    if (rows < 0 || cols < 1) return 0;
+    return (size_t)col_parts(rows, cols) * 2 * (size_t)cols * sizeof(float);
+}
+
+extern "C" int gnnx_layer_norm_backward(const gnnx_norm* n, const gnnx_drop* drop, void* workspace, size_t workspace_bytes, void* stream) {
+    NormArgs a;
+    if (const char* e = norm_args(n, &a)) return set_error(e);
+    if (const char* e = drop_args(drop, &a.drop)) return set_error(e);
+    if (!a.dx && !a.dw && !a.db) return 0;
+    if (a.rows > 0 && (a.dd != nullptr) != (drop != nullptr)) return set_error("layer norm: the gradient of a dropped output and its dropout go together");
+    if (a.rows > 0 && ((!a.dy && !a.dd) || !a.x || !a.mean || !a.rstd)) return set_error("null argument");
+    if (a.dw || a.db) {
+        if (!workspace || workspace_bytes < gnnx_layer_norm_workspace_bytes(n->type, a.rows, a.cols)) return set_error("workspace too small");
+        a.part = static_cast<float*>(workspace);
+        a.parts = col_parts(a.rows, a.cols);
+    }
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (n->type == GNNX_F32) a.dd ? run_backward<float, true>(a, s) : run_backward<float, false>(a, s);
+    else if (n->type == GNNX_BF16) a.dd ? run_backward<bf16_t, true>(a, s) : run_backward<bf16_t, false>(a, s);
+    else a.dd ? run_backward<f16_t, true>(a, s) : run_backward<f16_t, false>(a, s);
+    return launched("gnnx_layer_norm_backward");
+}
+
+extern "C" int gnnx_dropout(int32_t type, int64_t rows, int64_t cols, const void* x, int64_t x_stride, void* y, const gnnx_drop* drop, void* stream) {
+    DropArgs d;
+    if (type < 0 || type > 2) return set_error("dropout: type must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+    if (!drop) return set_error("null argument");
+    if (const char* e = drop_args(drop, &d)) return set_error(e);
+    if (rows < 0 || cols < 0 || x_stride < 0 || cols >= (int64_t(1) << 34)) return set_error("dropout: needs rows, stride >= 0 and 0 <= cols < 2^34");
+    if (rows == 0 || cols == 0) return 0;
+    if (!x || !y) return set_error("null argument");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const dim3 grid(grid_of(rows * ((cols + 3) / 4), 256)), block(256);
+    if (type == GNNX_F32) hipLaunchKernelGGL((k_dropout<float>), grid, block, 0, s, rows, cols, x_stride, static_cast<const float*>(x), static_cast<float*>(y), d);
+    else if (type == GNNX_BF16) hipLaunchKernelGGL((k_dropout<bf16_t>), grid, block, 0, s, rows, cols, x_stride, static_cast<const bf16_t*>(x), static_cast<bf16_t*>(y), d);
+    else hipLaunchKernelGGL((k_dropout<f16_t>), grid, block, 0, s, rows, cols, x_stride, static_cast<const f16_t*>(x), static_cast<f16_t*>(y), d);
+    return launched("gnnx_dropout");
+}

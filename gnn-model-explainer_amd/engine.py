@@ -75,6 +75,17 @@ class _XlState(ctypes.Structure):
                 ("m_out_e", ctypes.c_void_p), ("v_out_e", ctypes.c_void_p), ("feat_out", ctypes.c_void_p)]
 
 
+class _Drop(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("state", ctypes.c_void_p), ("row_offset", ctypes.c_int64), ("step", ctypes.c_uint32)]
+
+
+class _Norm(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("w_is_f32", ctypes.c_int32)] + \
+               [(k, ctypes.c_int64) for k in ("rows", "cols", "x_stride", "dy_stride", "dd_stride")] + \
+               [(k, ctypes.c_void_p) for k in ("x", "w", "b", "dy", "dd", "y", "d", "dx", "dw", "db", "mean", "rstd")] + \
+               [("eps", ctypes.c_float), ("relu", ctypes.c_int32)]
+
+
 @dataclass
 class AdamState:
     """Optimiser state of a batch (gnnx_resume, include/gnnx.h): what torch.optim.Adam keeps for ExplainModule's two
@@ -196,6 +207,11 @@ _API = {
     "gnnx_set_mt_jump_poly": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64]),
     "gnnx_set_mt_jump_polys": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32]),
     "gnnx_xl_run": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(_Hyper), ctypes.POINTER(_XlState)] + [ctypes.c_void_p] * 5),
+    "gnnx_layer_norm_forward": (ctypes.c_int, [ctypes.POINTER(_Norm), ctypes.POINTER(_Drop), ctypes.c_void_p]),
+    "gnnx_layer_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int64, ctypes.c_int64]),
+    "gnnx_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(_Norm), ctypes.POINTER(_Drop), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "gnnx_dropout": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.POINTER(_Drop),
+                                    ctypes.c_void_p]),
     "gnnx_last_error": (ctypes.c_char_p, []),
     "gnnx_version": (ctypes.c_char_p, []),
 }
@@ -241,6 +257,8 @@ def model_arrays(state_dict):
     extra = [k for k in state_dict if k.startswith("conv_block.") and not k.startswith("conv_block.0.")]
     if extra:
         raise NotImplementedError("the HIP path implements num_gc_layers == 3 (one conv_block), got " + str(extra))
+    if any(k.startswith("norms.") for k in state_dict):
+        raise NotImplementedError("the HIP path implements encoders without layer norm (models.LayerNorm): the PyTorch-ROCm route explains those")
     out = {}
     for k in STATE_KEYS:
         if k not in state_dict:

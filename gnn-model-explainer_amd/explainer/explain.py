@@ -151,6 +151,8 @@ def _torch_route_reason(args, model, state_dict=None, graph_mode=False, record_l
     extra = [k for k in sd if k.startswith("conv_block.") and not k.startswith("conv_block.0.")]
     if extra or "conv_block.0.weight" not in sd:
         return "an encoder with %d graph-convolution layers (the kernels implement 3)" % (2 + len({k.split(".")[1] for k in sd if k.startswith("conv_block.")}))
+    if any(k.startswith("norms.") for k in sd):
+        return "an encoder with layer norm"
     if any(k.endswith("self_weight") for k in sd):
         return "an encoder with add_self"
     if "pred_model.weight" not in sd or "conv_first.bias" not in sd:

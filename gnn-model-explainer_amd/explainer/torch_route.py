@@ -1,6 +1,6 @@
 """The PyTorch-ROCm route for the configurations the HIP kernels do not implement ("fall back to a
 PyTorch-ROCm restatement of the reference path rather than silently differ"): `model="att"` (the attention baseline),
-`num_gc_layers != 3`, encoders with `add_self` / dropout / a hidden prediction head, node explanations on a graph-mode Explainer,
+`num_gc_layers != 3`, encoders with `add_self` / dropout / layer norm / a hidden prediction head, node explanations on a graph-mode Explainer,
 `method="att"` together with `--bn` / a ReLU mask / loss logging / unconstrained (`method="att"` itself runs on k_att), and
 `ExplainModule.forward(marginalize=True / mask_features=False)`.
 
@@ -110,6 +110,8 @@ def explain_one(model, sub_adj, sub_feat, sub_label, pred_label, node_idx_new, a
     sched, opt = make_optimizer(args, params)
     model.eval()
     mod.train()                      # explain.py:135: this flips the wrapped model to train mode too (dropout)
+    if hasattr(model, "reset_dropout"):      # counter-based dropout: the same masks for this target whatever was explained before it
+        model.reset_dropout()
     adj_atts = None
     for _ in range(int(args.num_epochs)):
         mod.zero_grad()

@@ -42,6 +42,9 @@ def arg_parse(argv=None):
     parser.add_argument("--num-gc-layers", dest="num_gc_layers", type=int)
     parser.add_argument("--bn", dest="bn", action="store_const", const=True, default=False)
     parser.add_argument("--dropout", dest="dropout", type=float)
+    parser.add_argument("--dropout-seed", dest="dropout_seed", type=int, help="Apply --dropout in the encoder, masks drawn from this seed (ops.dropout).")
+    parser.add_argument("--layer-norm", dest="layer_norm", action="store_const", const=True, default=False,
+                        help="The encoder has a LayerNorm after every hidden layer.")
     parser.add_argument("--nobias", dest="bias", action="store_const", const=False, default=True)
     parser.add_argument("--no-writer", dest="writer", action="store_const", const=False, default=True)
     parser.add_argument("--mask-act", dest="mask_act", type=str, help="sigmoid, ReLU.")
@@ -75,7 +78,8 @@ def main(argv=None):
     graph_mode = prog_args.graph_mode or prog_args.multigraph_class >= 0 or prog_args.graph_idx >= 0
     cls = models.GcnEncoderGraph if graph_mode else models.GcnEncoderNode
     model = cls(input_dim=input_dim, hidden_dim=prog_args.hidden_dim, embedding_dim=prog_args.output_dim,
-                label_dim=num_classes, num_layers=prog_args.num_gc_layers, bn=prog_args.bn, args=prog_args)
+                label_dim=num_classes, num_layers=prog_args.num_gc_layers, bn=prog_args.bn,
+                dropout=prog_args.dropout if prog_args.dropout_seed is not None else 0.0, args=prog_args)
     model.load_state_dict(ckpt["model_state"])
     explainer = explain.Explainer(model=model, adj=cg_dict["adj"], feat=cg_dict["feat"], label=cg_dict["label"],
                                   pred=cg_dict["pred"], train_idx=cg_dict["train_idx"], args=prog_args, writer=None,

@@ -6,21 +6,64 @@ The HIP engine reads only the frozen weights of the default configuration (3 lay
 `forward` is a plain torch restatement of the reference's forward: predictions outside the hot path, and the model the torch
 route of the explainer (explainer/torch_route.py) differentiates through for the configurations the kernels do not implement -
 `method="att"` (models.py:62-68: adj * (x W_att)(x W_att)^T per layer), any number of layers, `add_self`, dropout.
+
+Two options the reference does not have, both read from `args`, both on the kernels of ops.py where the model is on the GPU:
+  layer_norm    True: a learned LayerNorm after the ReLU of every hidden layer in the place of apply_bn (state_dict keys norms.<layer>.weight / .bias);
+  dropout_seed  an int: the layers' dropout draws its masks from (seed, use, layer, node, feature) instead of torch's generator, so that a training run or an
+                explanation through the torch route is reproducible by itself; `reset_dropout()` starts the uses again.
 """
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import ops
+
+
+class LayerNorm(nn.Module):
+    """LayerNorm over the features of relu(x), one gain and offset per feature; on the GPU one kernel (ops.layer_norm), the ReLU in it."""
+
+    def __init__(self, dim, eps=1e-5):
+        super().__init__()
+        self.dim, self.eps = dim, eps
+        self.weight = nn.Parameter(torch.ones(dim))
+        self.bias = nn.Parameter(torch.zeros(dim))
+
+    def forward(self, x):
+        if x.is_cuda or ops._ENGINE["lib"] is not None:
+            return ops.layer_norm(x, self.weight, self.bias, self.eps, relu=True)
+        return F.layer_norm(F.relu(x), (self.dim,), self.weight, self.bias, self.eps)
+
+    def with_dropout(self, x, drop):
+        """(self(x), drop(self(x))) in one pass each way (ops.layer_norm_dropout)."""
+        return ops.layer_norm_dropout(x, self.weight, self.bias, drop.p, drop.seed, drop.next_step(), self.eps, relu=True)
+
+
+class CounterDropout(nn.Module):
+    """Dropout whose mask is a function of (seed, use, layer, row, feature): ops.dropout.  `uses` counts the calls in training mode."""
+
+    def __init__(self, p, seed, layer, layers):
+        super().__init__()
+        self.p, self.seed, self.layer, self.layers, self.uses = float(p), int(seed), layer, layers, 0
+
+    def next_step(self):
+        step = self.uses * self.layers + self.layer
+        self.uses += 1
+        return step
+
+    def forward(self, x):
+        return ops.dropout(x, self.p, self.seed, self.next_step()) if self.training else x
+
 
 class GraphConv(nn.Module):
     """y = normalize((adj' x) W (+ x W_self) + b), adj' = adj * att with att = (x W_att)(x W_att)^T when `att` (models.py:58-80)."""
 
-    def __init__(self, input_dim, output_dim, add_self=False, normalize_embedding=False, dropout=0.0, bias=True, gpu=True, att=False):
+    def __init__(self, input_dim, output_dim, add_self=False, normalize_embedding=False, dropout=0.0, bias=True, gpu=True, att=False,
+                 dropout_layer=None):
         super().__init__()
         self.att, self.add_self, self.dropout, self.normalize_embedding = att, add_self, dropout, normalize_embedding
         self.input_dim, self.output_dim = input_dim, output_dim
         if dropout > 0.001:
-            self.dropout_layer = nn.Dropout(p=dropout)
+            self.dropout_layer = nn.Dropout(p=dropout) if dropout_layer is None else dropout_layer
         self.weight = nn.Parameter(torch.empty(input_dim, output_dim))
         if add_self:
             self.self_weight = nn.Parameter(torch.empty(input_dim, output_dim))
@@ -28,8 +71,14 @@ class GraphConv(nn.Module):
             self.att_weight = nn.Parameter(torch.empty(input_dim, input_dim))
         self.bias = nn.Parameter(torch.zeros(output_dim)) if bias else None
 
-    def forward(self, x, adj):
-        if self.dropout > 0.001:
+    def counter_dropout(self):
+        """The layer's CounterDropout where it is to be applied now, else None."""
+        drop = self.dropout_layer if self.dropout > 0.001 else None
+        return drop if isinstance(drop, CounterDropout) and drop.training else None
+
+    def forward(self, x, adj, dropped=False):
+        """dropped: x has been through this layer's dropout already (LayerNorm.with_dropout)."""
+        if self.dropout > 0.001 and not dropped:
             x = self.dropout_layer(x)
         if self.att:
             x_att = torch.matmul(x, self.att_weight)
@@ -51,10 +100,18 @@ class GcnEncoderGraph(nn.Module):
         self.concat, self.bn, self.num_layers, self.num_aggs = concat, bool(bn), num_layers, 1
         self.bias = True if args is None else getattr(args, "bias", True)
         self.att = args is not None and getattr(args, "method", "base") == "att"
-        gc = lambda i, o, dp=0.0: GraphConv(i, o, add_self=add_self, normalize_embedding=True, dropout=dp, bias=self.bias, att=self.att)
+        seed = None if args is None else getattr(args, "dropout_seed", None)
+        counter = lambda layer: None if seed is None or not dropout > 0.001 else CounterDropout(dropout, seed, layer, num_layers - 2)
+        gc = lambda i, o, dp=0.0, drop=None: GraphConv(i, o, add_self=add_self, normalize_embedding=True, dropout=dp, bias=self.bias, att=self.att,
+                                                       dropout_layer=drop)
         self.conv_first = gc(input_dim, hidden_dim)
-        self.conv_block = nn.ModuleList([gc(hidden_dim, hidden_dim, dropout) for _ in range(num_layers - 2)])
+        self.conv_block = nn.ModuleList([gc(hidden_dim, hidden_dim, dropout, counter(i)) for i in range(num_layers - 2)])
         self.conv_last = gc(hidden_dim, embedding_dim)
+        self.norms = None
+        if args is not None and getattr(args, "layer_norm", False):
+            if self.bn:
+                raise ValueError("bn and layer_norm are two normalisations of the same rows: choose one")
+            self.norms = nn.ModuleList([LayerNorm(hidden_dim) for _ in range(num_layers - 1)])
         self.act = nn.ReLU()
         self.label_dim = label_dim
         self.pred_input_dim = hidden_dim * (num_layers - 1) + embedding_dim if concat else embedding_dim
@@ -80,43 +137,54 @@ class GcnEncoderGraph(nn.Module):
         """models.py:222-228: a fresh BatchNorm1d(num_nodes) in training mode - every node standardised over its features."""
         return F.batch_norm(x, None, None, None, None, True, 0.1, 1e-5)
 
-    def gcn_forward(self, x, adj):
-        """models.py:230-267: all layers, concatenated embeddings [1, n, H (L - 1) + O] and the stacked attention adjacencies (the
-        block layers re-append conv_first's, as the reference does at :252)."""
-        x, adj_att = self.conv_first(x, adj)
+    def reset_dropout(self):
+        """Every CounterDropout starts its uses again: what follows draws the masks that a new model would."""
+        for m in self.modules():
+            if isinstance(m, CounterDropout):
+                m.uses = 0
+
+    def _activate(self, layer, x, nxt):
+        """What follows graph convolution `layer` (models.py:239-253): (the layer's embedding, what convolution `nxt` reads, whether that has been through its
+        dropout)."""
+        if self.norms is not None:
+            drop = nxt.counter_dropout()
+            if drop is not None:
+                h, d = self.norms[layer].with_dropout(x, drop)
+                return h, d, True
+            x = self.norms[layer](x)
+            return x, x, False
         x = self.act(x)
         if self.bn:
             x = self.apply_bn(x)
-        x_all, att_all = [x], [adj_att]
-        for conv in self.conv_block:
-            x, _ = conv(x, adj)
-            x = self.act(x)
-            if self.bn:
-                x = self.apply_bn(x)
-            x_all.append(x)
-            att_all.append(adj_att)
-        x, adj_att = self.conv_last(x, adj)
-        x_all.append(x)
-        att_all.append(adj_att)
+        return x, x, False
+
+    def _layers(self, x, adj):
+        """The graph convolutions one after the other: (embedding, attention adjacency) of each."""
+        convs = [self.conv_first, *self.conv_block, self.conv_last]
+        dropped = False
+        for i, conv in enumerate(convs):
+            x, adj_att = conv(x, adj, dropped)
+            if i + 1 == len(convs):
+                yield x, adj_att
+                return
+            h, x, dropped = self._activate(i, x, convs[i + 1])
+            yield h, adj_att
+
+    def gcn_forward(self, x, adj):
+        """models.py:230-267: all layers, concatenated embeddings [1, n, H (L - 1) + O] and the stacked attention adjacencies (the
+        block layers re-append conv_first's, as the reference does at :252)."""
+        x_all, att_all = [], []
+        for i, (h, adj_att) in enumerate(self._layers(x, adj)):
+            x_all.append(h)
+            att_all.append(att_all[0] if 0 < i <= len(self.conv_block) else adj_att)
         return torch.cat(x_all, dim=2), torch.stack(att_all, dim=3)
 
     def forward(self, x, adj, batch_num_nodes=None, **kwargs):
         """models.py:269-316: per-layer max over all rows, concat, linear head."""
-        x, adj_att = self.conv_first(x, adj)
-        x = self.act(x)
-        if self.bn:
-            x = self.apply_bn(x)
-        outs, atts = [x.max(dim=1)[0]], [adj_att]
-        for conv in self.conv_block:
-            x, adj_att = conv(x, adj)
-            x = self.act(x)
-            if self.bn:
-                x = self.apply_bn(x)
-            outs.append(x.max(dim=1)[0])
+        outs, atts = [], []
+        for h, adj_att in self._layers(x, adj):
+            outs.append(h.max(dim=1)[0])
             atts.append(adj_att)
-        x, adj_att = self.conv_last(x, adj)
-        atts.append(adj_att)
-        outs.append(x.max(dim=1)[0])
         output = torch.cat(outs, dim=1) if self.concat else outs[-1]
         return self.pred_model(output), torch.stack(atts, dim=3)
 

@@ -413,6 +413,55 @@ int gnnx_xl_set_clocks(gnnx_xl_handle h, int64_t* ticks);
 int gnnx_xl_run(gnnx_xl_handle h, const gnnx_hyper* hyper, const gnnx_xl_state* state, float* abar_e, float* feat_mask, void* ws_rows,
                 void* ws_entries, void* stream);
 
+/* ---- operators of an encoder's layers (csrc/gnnx_norm.hpp, csrc/gnnx_ops.hip) ----
+ * What stands between two graph convolutions of an encoder (models.py:58-61, 230-267): layer norm with the ReLU before it, dropout, and the two in one pass,
+ * each with its backward pass.  Matrices of `rows` rows and `cols` columns: the elements of a row contiguous, the rows of an INPUT its stride apart
+ * (in elements; 0: every row the same), outputs contiguous; DEVICE pointers, aligned to their element; asynchronous on `stream`, which belongs to the current
+ * device.  Nothing is kept between calls, no call synchronises, allocates or clears memory through the runtime: all of them can be captured into a graph. */
+#define GNNX_F32 0
+#define GNNX_BF16 1
+#define GNNX_F16 2
+
+/* Dropout whose mask is a function of (seed, step, row, column): an element stays, scaled by 1 / (1 - p), where its 32-bit word is >= round(p 2^32); it is 0
+ * otherwise, whatever it was (infinities and NaN included).  word(r, c) = word c mod 4 of Philox-4x32-10 (Salmon, Moraes, Dror, Shaw, SC 2011) at counter
+ * (c / 4, r mod 2^32, r / 2^32, step) under the key (seed mod 2^32, seed / 2^32), r = row_offset + the row of this call. */
+typedef struct {
+    double p;             /* in [0, 1] */
+    uint64_t seed;
+    const int64_t* state; /* DEVICE [2] = (seed, step) read when the kernel runs, or NULL: what a captured graph needs; `seed` is then unused, `step` is added */
+    int64_t row_offset;   /* the row of the whole tensor that row 0 of this call is (a shard's) */
+    uint32_t step;
+} gnnx_drop;
+
+/* v = relu ? max(x, 0) : x;  mean, rstd = 1 / sqrt(variance + eps) over a row of v;  y = (v - mean) rstd w + b;  d = dropout(y).  fp32 arithmetic. */
+typedef struct {
+    int32_t type;                           /* GNNX_F32 / GNNX_BF16 / GNNX_F16: x, y, d, dy, dd, dx */
+    int32_t w_is_f32;                       /* 1: w, b, dw, db are fp32; 0: they have x's type */
+    int64_t rows, cols;                     /* cols < 2^30 */
+    int64_t x_stride, dy_stride, dd_stride;
+    const void* x;
+    const void* w;                          /* [cols] or NULL = 1 */
+    const void* b;                          /* [cols] or NULL = 0 */
+    const void* dy;                         /* backward: gradient of y, or NULL = 0 */
+    const void* dd;                         /* backward: gradient of d, or NULL (then no gnnx_drop either) */
+    void* y;                                /* forward out, or NULL */
+    void* d;                                /* forward out, or NULL (then no gnnx_drop either) */
+    void* dx;                               /* backward out, or NULL */
+    void* dw;                               /* backward out [cols], or NULL */
+    void* db;                               /* backward out [cols], or NULL */
+    float* mean;                            /* [rows]: forward out (or NULL, with rstd), backward in */
+    float* rstd;
+    float eps;                              /* >= 0 (forward) */
+    int32_t relu;                           /* backward: dx = 0 where x <= 0 */
+} gnnx_norm;
+int gnnx_layer_norm_forward(const gnnx_norm* n, const gnnx_drop* drop, void* stream);
+/* workspace: DEVICE scratch of gnnx_layer_norm_workspace_bytes(type, rows, cols) bytes, or NULL where neither dw nor db is asked for.  dw and db are summed in
+ * an order that the sizes alone decide: the same inputs give the same bits. */
+size_t gnnx_layer_norm_workspace_bytes(int32_t type, int64_t rows, int64_t cols);
+int gnnx_layer_norm_backward(const gnnx_norm* n, const gnnx_drop* drop, void* workspace, size_t workspace_bytes, void* stream);
+/* y = dropout(x), y contiguous; its backward pass is the same call on the gradient. */
+int gnnx_dropout(int32_t type, int64_t rows, int64_t cols, const void* x, int64_t x_stride, void* y, const gnnx_drop* drop, void* stream);
+
 const char* gnnx_last_error(void);
 const char* gnnx_version(void);
 

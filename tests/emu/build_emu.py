@@ -17,7 +17,9 @@ def build(force=False):
             os.path.join(HERE, "emu_runtime.cpp"), os.path.join(HERE, "include", "hip", "hip_runtime.h"),
             os.path.join(ROOT, "include", "gnnx.h"), os.path.join(CSRC, "gnnx_resident.hpp"),
             os.path.join(CSRC, "gnnx_sparse.hpp"), os.path.join(CSRC, "gnnx_sparse_large.hpp"),
-            os.path.join(CSRC, "gnnx_graph.hpp"), os.path.join(CSRC, "gnnx_att.hpp"), os.path.join(CSRC, "gnnx_xl.hpp")]
+            os.path.join(CSRC, "gnnx_graph.hpp"), os.path.join(CSRC, "gnnx_att.hpp"), os.path.join(CSRC, "gnnx_xl.hpp"),
+            os.path.join(CSRC, "gnnx_ops.hip"), os.path.join(CSRC, "gnnx_norm.hpp"), os.path.join(CSRC, "gnnx_error.hpp")]
+    units = [s for s in srcs if s.endswith((".hip", ".cpp"))]
     fresh = lambda: os.path.exists(OUT) and all(os.path.getmtime(OUT) >= os.path.getmtime(s) for s in srcs)
     if not force and fresh():
         return OUT
@@ -30,10 +32,19 @@ def build(force=False):
         cxx = "/opt/rocm/lib/llvm/bin/clang++"
         if not os.path.exists(cxx):
             cxx = "clang++"
+        objs, running = [], []
+        for u in units:      # side by side; the flags are one set for all
+            objs.append(os.path.join(HERE, "_build", os.path.basename(u) + ".%d.o" % os.getpid()))
+            cmd = [cxx, "-O2", "-g", "-std=c++17", "-fPIC", "-ffp-contract=on", "-Wno-psabi", "-I", os.path.join(HERE, "include"), "-x", "c++", "-c", u,
+                   "-o", objs[-1]]
+            running.append((cmd, subprocess.Popen(cmd)))
+        for cmd, proc in running:
+            if proc.wait() != 0:
+                raise subprocess.CalledProcessError(proc.returncode, cmd)
         tmp = OUT + ".tmp%d" % os.getpid()
-        cmd = [cxx, "-O2", "-g", "-std=c++17", "-shared", "-fPIC", "-ffp-contract=on", "-Wno-psabi", "-I", os.path.join(HERE, "include"),
-               "-x", "c++", srcs[0], srcs[2], "-o", tmp]
-        subprocess.check_call(cmd)
+        subprocess.check_call([cxx, "-shared", "-fPIC"] + objs + ["-o", tmp])
+        for o in objs:
+            os.remove(o)
         os.replace(tmp, OUT)      # never a half-written library under the final name
     return OUT
 
