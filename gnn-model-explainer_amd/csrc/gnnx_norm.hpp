@@ -70,51 +70,283 @@ __device__ __forceinline__ float dropped(const DropArgs& a, uint32_t word, float
     return word > a.last_dropped || !a.on ? v * a.scale : 0.0f;
 }
 
-__device__ __forceinline__ float wave_total(float v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-    return v;
-}
+__device__ __forceinline__ float floored(float v, float floor) { return v < floor ? floor : v; }      // ReLU (floor 0) or nothing (floor -inf); NaN stays
 
 template <class T>
 __device__ __forceinline__ float param_at(const void* p, int32_t is_f32, int64_t c) {
     return is_f32 ? static_cast<const float*>(p)[c] : (float)static_cast<const T*>(p)[c];
 }
 
-// One wave per row, the row read again for each of the three passes (mean, squared distance from it, output).
+// ---- a row in registers ----
+// A row is shared by TPR lanes (beyond 64: threads of a workgroup); each holds K pieces of 16 bytes, V elements.  Piece k of lane l is meant to start at column
+// (k TPR + l) V; one that would reach past the row starts at cols - V instead and leaves out of every sum the `skip` elements that the piece before it has as
+// well (a piece wholly beyond the row leaves out all V).  So every access is one 16-byte access inside the row, whatever the row's length and alignment (the
+// hardware takes any alignment): no tail, no variant for odd rows or slices.  Both holders of an element store the same value.  Needs cols >= V.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <class T>
+struct Piece {
+    static constexpr int V = 16 / (int)sizeof(T);
+    u32x4 w;
+    __device__ __forceinline__ float at(int j) const {
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, +w[j]);      // (+: of the lane's value; a cast of the vector's lane itself reads lane 0)
+        else if constexpr (__is_same(T, bf16_t)) return __builtin_bit_cast(float, j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+        else return (float)__builtin_bit_cast(f16_t, (uint16_t)(j & 1 ? w[j >> 1] >> 16 : w[j >> 1]));
+    }
+};
+template <class T>
+__device__ __forceinline__ Piece<T> load_piece(const T* p) {
+    Piece<T> q;
+    __builtin_memcpy(&q.w, p, 16);
+    return q;
+}
+template <class T>
+__device__ __forceinline__ void store_piece(T* p, const float* v) {
+    Piece<T> q;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q.w[j] = __builtin_bit_cast(uint32_t, v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            q.w[j] = (uint32_t)__builtin_bit_cast(uint16_t, (T)v[2 * j]) | (uint32_t)__builtin_bit_cast(uint16_t, (T)v[2 * j + 1]) << 16;
+    }
+    __builtin_memcpy(p, &q.w, 16);
+}
+// the V parameters of a piece (fp32, or x's type)
+template <class T>
+__device__ __forceinline__ void load_params(float* out, const void* p, int32_t is_f32, int64_t c) {
+    constexpr int V = Piece<T>::V;
+    if (sizeof(T) == 4 || is_f32) {
+#pragma unroll
+        for (int h = 0; h < V; h += 4) {
+            const Piece<float> q = load_piece(static_cast<const float*>(p) + c + h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[h + j] = q.at(j);
+        }
+    } else {
+        const Piece<T> q = load_piece(static_cast<const T*>(p) + c);
+#pragma unroll
+        for (int j = 0; j < V; ++j) out[j] = q.at(j);
+    }
+}
+struct Slot { int64_t c; int skip; };
+template <int V>
+__device__ __forceinline__ Slot slot_at(int64_t c, int64_t cols) {
+    const int64_t last = cols - V, over = c - last;
+    return over <= 0 ? Slot{c, 0} : Slot{last, over < V ? (int)over : V};
+}
+
+// The dropout of a piece's V elements from column c on (c is a multiple of 4 unless the piece was moved back from the end of a row that 4 does not divide:
+// its words then lie across V / 4 + 1 blocks).
+template <class T>
+__device__ __forceinline__ void drop_piece(const DropArgs& d, const DropKey& key, int64_t r, int64_t c, int64_t cols, float* v) {
+    constexpr int V = Piece<T>::V;
+    if ((cols & 3) == 0) {
+#pragma unroll
+        for (int h = 0; h < V; h += 4) {
+            const Philox4 q = drop_words(d, key, r, (uint32_t)(c >> 2) + h / 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[h + j] = dropped(d, q.w[j], v[h + j]);
+        }
+    } else {
+        uint32_t w[V + 4];
+#pragma unroll
+        for (int h = 0; h < V + 4; h += 4) {
+            const Philox4 q = drop_words(d, key, r, (uint32_t)(c >> 2) + h / 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[h + j] = q.w[j];
+        }
+        const int sh = (int)(c & 3);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const uint32_t lo = sh & 1 ? w[j + 1] : w[j], hi = sh & 1 ? w[j + 3] : w[j + 2];
+            v[j] = dropped(d, sh & 2 ? hi : lo, v[j]);
+        }
+    }
+}
+
+// Sums over the TPR lanes that share a row, in every one of them; beyond a wave through `part` (one float per wave and sum).
+template <int TPR, int N>
+__device__ __forceinline__ void row_totals(float (&v)[N], float (*part)[N]) {
+#pragma unroll
+    for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
+    if constexpr (TPR > 64) {
+        constexpr int W = TPR / 64;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) part[threadIdx.x >> 6][i] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) s += part[w][i];
+            v[i] = s;
+        }
+    }
+}
+
+// y (and d) of one piece from its xhat
 template <class T, bool DROP>
-__global__ __launch_bounds__(256) void k_norm_forward(NormArgs a) {
-    const int lane = threadIdx.x & 63;
+__device__ __forceinline__ void norm_outputs(const NormArgs& a, const DropKey& key, int64_t r, int64_t c, float* v) {
+    constexpr int V = Piece<T>::V;
+    float p[V];
+    if (a.w) {
+        load_params<T>(p, a.w, a.w_is_f32, c);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] *= p[j];
+    }
+    if (a.b) {
+        load_params<T>(p, a.b, a.w_is_f32, c);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] += p[j];
+    }
+    if (a.y) store_piece(static_cast<T*>(a.y) + r * a.cols + c, v);
+    if (DROP) {
+        drop_piece<T>(a.drop, key, r, c, a.cols, v);
+        store_piece(static_cast<T*>(a.d) + r * a.cols + c, v);
+    }
+}
+
+template <int TPR>
+constexpr int norm_threads() { return TPR <= 64 ? 256 : TPR; }
+
+template <class T, int TPR, int K, bool DROP>
+__global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a) {
+    constexpr int V = Piece<T>::V, RPB = norm_threads<TPR>() / TPR;
+    __shared__ float part[2][TPR > 64 ? TPR / 64 : 1][1];
+    const int l = threadIdx.x % TPR;
     const float inv = 1.0f / (float)a.cols;
     const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * 4) {
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
+        const bool live = r0 + threadIdx.x / TPR < a.rows;      // (a workgroup of one row is live as a whole)
+        const int64_t r = live ? r0 + threadIdx.x / TPR : a.rows - 1;
         const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
-        float s = 0.0f;
-        for (int64_t c = lane; c < a.cols; c += 64) {
-            const float v = (float)x[c];
-            s += v < a.relu_floor ? a.relu_floor : v;
+        Piece<T> q[K];                             // as stored: widened again in each pass, half the registers for 16-bit types
+        Slot at[K];
+        float s[1] = {0.0f};
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            at[k] = slot_at<V>((k * TPR + l) * V, a.cols);
+            q[k] = load_piece(x + at[k].c);
         }
-        const float mean = wave_total(s) * inv;
-        s = 0.0f;
-        for (int64_t c = lane; c < a.cols; c += 64) {
-            float v = (float)x[c];
-            v = (v < a.relu_floor ? a.relu_floor : v) - mean;
-            s += v * v;
-        }
-        const float rstd = 1.0f / sqrtf(wave_total(s) * inv + a.eps);
-        if (lane == 0 && a.mean) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float v = floored(q[k].at(j), a.relu_floor);
+                s[0] += 2 * k + 1 < K || j >= at[k].skip ? v : 0.0f;      // (more than half of the K rounds are full: run_forward)
+            }
+        row_totals<TPR>(s, part[0]);
+        const float mean = s[0] * inv;
+        s[0] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float v = floored(q[k].at(j), a.relu_floor) - mean;
+                s[0] += 2 * k + 1 < K || j >= at[k].skip ? v * v : 0.0f;
+            }
+        row_totals<TPR>(s, part[1]);
+        const float rstd = 1.0f / sqrtf(s[0] * inv + a.eps);
+        if (!live) continue;
+        if (l == 0 && a.mean) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
         }
-        for (int64_t c = lane; c < a.cols; c += 64) {
-            float v = (float)x[c];
-            v = ((v < a.relu_floor ? a.relu_floor : v) - mean) * rstd;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (at[k].skip < V) {
+                float v[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] = (floored(q[k].at(j), a.relu_floor) - mean) * rstd;
+                norm_outputs<T, DROP>(a, key, r, at[k].c, v);
+            }
+        }
+    }
+}
+
+// Rows too long for registers: one workgroup per row, the row read again for each of the three passes (mean, squared distance from it, output).
+template <class T, bool DROP>
+__global__ __launch_bounds__(1024) void k_norm_forward_long(NormArgs a) {
+    constexpr int V = Piece<T>::V;
+    __shared__ float part[2][16][1];
+    const float inv = 1.0f / (float)a.cols;
+    const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
+        float s[1] = {0.0f};
+        for (int64_t c = (int64_t)threadIdx.x * V; c < a.cols; c += 1024 * V) {
+            const Slot t = slot_at<V>(c, a.cols);
+            const Piece<T> q = load_piece(x + t.c);
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[0] += j >= t.skip ? floored(q.at(j), a.relu_floor) : 0.0f;
+        }
+        row_totals<1024>(s, part[0]);
+        const float mean = s[0] * inv;
+        s[0] = 0.0f;
+        for (int64_t c = (int64_t)threadIdx.x * V; c < a.cols; c += 1024 * V) {
+            const Slot t = slot_at<V>(c, a.cols);
+            const Piece<T> q = load_piece(x + t.c);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float v = floored(q.at(j), a.relu_floor) - mean;
+                s[0] += j >= t.skip ? v * v : 0.0f;
+            }
+        }
+        row_totals<1024>(s, part[1]);
+        const float rstd = 1.0f / sqrtf(s[0] * inv + a.eps);
+        if (threadIdx.x == 0 && a.mean) {
+            a.mean[r] = mean;
+            a.rstd[r] = rstd;
+        }
+        for (int64_t c = (int64_t)threadIdx.x * V; c < a.cols; c += 1024 * V) {
+            const Slot t = slot_at<V>(c, a.cols);
+            const Piece<T> q = load_piece(x + t.c);
+            float v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = (floored(q.at(j), a.relu_floor) - mean) * rstd;
+            norm_outputs<T, DROP>(a, key, r, t.c, v);
+        }
+    }
+}
+
+// Rows shorter than one piece (fewer than 4 or 8 columns): one thread per row.
+template <class T, bool DROP>
+__global__ __launch_bounds__(256) void k_norm_forward_narrow(NormArgs a) {
+    const float inv = 1.0f / (float)a.cols;
+    const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
+    for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < a.rows; r += (int64_t)gridDim.x * 256) {
+        const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
+        float s = 0.0f;
+        for (int c = 0; c < a.cols; ++c) s += floored((float)x[c], a.relu_floor);
+        const float mean = s * inv;
+        s = 0.0f;
+        for (int c = 0; c < a.cols; ++c) {
+            const float v = floored((float)x[c], a.relu_floor) - mean;
+            s += v * v;
+        }
+        const float rstd = 1.0f / sqrtf(s * inv + a.eps);
+        if (a.mean) {
+            a.mean[r] = mean;
+            a.rstd[r] = rstd;
+        }
+        for (int c = 0; c < a.cols; ++c) {
+            float v = (floored((float)x[c], a.relu_floor) - mean) * rstd;
             if (a.w) v *= param_at<T>(a.w, a.w_is_f32, c);
             if (a.b) v += param_at<T>(a.b, a.w_is_f32, c);
             if (a.y) static_cast<T*>(a.y)[r * a.cols + c] = (T)v;
             if (DROP) static_cast<T*>(a.d)[r * a.cols + c] = (T)dropped(a.drop, drop_words(a.drop, key, r, (uint32_t)(c >> 2)).w[c & 3], v);
         }
     }
+}
+
+__device__ __forceinline__ float wave_total(float v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    return v;
 }
 
 // dL/dy at (r, c): the gradient of the kept output plus that of the dropped one

@@ -22,10 +22,10 @@ int launched(const char* what) {
     return set_error(text);
 }
 
-// workgroups of a launch that walks `items` with a grid stride: at most 2^22 (256 threads each: the 32-bit work-item limit of a launch)
-unsigned grid_of(int64_t items, int64_t per_group) {
-    const int64_t g = (items + per_group - 1) / per_group;
-    return (unsigned)(g < 1 ? 1 : g > (int64_t(1) << 22) ? (int64_t(1) << 22) : g);
+// workgroups of a launch that walks `items` with a grid stride: at most 2^31 threads in all (the work-items of a launch are counted in 32 bits)
+unsigned grid_of(int64_t items, int64_t per_group, int64_t threads) {
+    const int64_t g = (items + per_group - 1) / per_group, most = (int64_t(1) << 31) / threads;
+    return (unsigned)(g < 1 ? 1 : g > most ? most : g);
 }
 
 const char* drop_args(const gnnx_drop* d, DropArgs* out) {
@@ -82,15 +82,36 @@ int col_parts(int64_t rows, int64_t cols) {
     return (int)(parts < 1 ? 1 : parts);
 }
 
-template <class T>
+template <class T, int TPR, int K, bool DROP>
+void forward_rows(const NormArgs& a, hipStream_t s) {
+    constexpr int NT = norm_threads<TPR>();
+    hipLaunchKernelGGL((k_norm_forward<T, TPR, K, DROP>), dim3(grid_of(a.rows, NT / TPR, NT)), dim3(NT), 0, s, a);
+}
+
+// The lanes of a row: as few as hold it with one piece each up to a wave, then two to eight pieces each before more waves join in.
+template <class T, bool DROP>
 void run_forward(const NormArgs& a, hipStream_t s) {
-    if (a.d) hipLaunchKernelGGL((k_norm_forward<T, true>), dim3(grid_of(a.rows, 4)), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_norm_forward<T, false>), dim3(grid_of(a.rows, 4)), dim3(256), 0, s, a);
+    const int64_t pieces = (a.cols + Piece<T>::V - 1) / Piece<T>::V;
+    if (a.cols < Piece<T>::V) hipLaunchKernelGGL((k_norm_forward_narrow<T, DROP>), dim3(grid_of(a.rows, 256, 256)), dim3(256), 0, s, a);
+    else if (pieces <= 1) forward_rows<T, 1, 1, DROP>(a, s);
+    else if (pieces <= 2) forward_rows<T, 2, 1, DROP>(a, s);
+    else if (pieces <= 4) forward_rows<T, 4, 1, DROP>(a, s);
+    else if (pieces <= 8) forward_rows<T, 8, 1, DROP>(a, s);
+    else if (pieces <= 16) forward_rows<T, 16, 1, DROP>(a, s);
+    else if (pieces <= 32) forward_rows<T, 32, 1, DROP>(a, s);
+    else if (pieces <= 64) forward_rows<T, 64, 1, DROP>(a, s);
+    else if (pieces <= 128) forward_rows<T, 64, 2, DROP>(a, s);
+    else if (pieces <= 256) forward_rows<T, 64, 4, DROP>(a, s);
+    else if (pieces <= 512) forward_rows<T, 256, 2, DROP>(a, s);
+    else if (pieces <= 1024) forward_rows<T, 256, 4, DROP>(a, s);
+    else if (pieces <= 2048) forward_rows<T, 1024, 2, DROP>(a, s);
+    else if (pieces <= 4096) forward_rows<T, 1024, 4, DROP>(a, s);
+    else hipLaunchKernelGGL((k_norm_forward_long<T, DROP>), dim3(grid_of(a.rows, 1, 1024)), dim3(1024), 0, s, a);
 }
 
 template <class T, bool DROP>
 void run_backward(const NormArgs& a, hipStream_t s) {
-    if (a.dx && a.rows) hipLaunchKernelGGL((k_norm_backward_rows<T, DROP>), dim3(grid_of(a.rows, 4)), dim3(256), 0, s, a);
+    if (a.dx && a.rows) hipLaunchKernelGGL((k_norm_backward_rows<T, DROP>), dim3(grid_of(a.rows, 4, 256)), dim3(256), 0, s, a);
     if (!a.dw && !a.db) return;
     const unsigned tiles = (unsigned)((a.cols + 63) / 64);
     hipLaunchKernelGGL((k_norm_backward_cols<T, DROP>), dim3(tiles * (unsigned)a.parts), dim3(256), 0, s, a);
@@ -109,9 +130,9 @@ extern "C" int gnnx_layer_norm_forward(const gnnx_norm* n, const gnnx_drop* drop
     if ((a.mean != nullptr) != (a.rstd != nullptr)) return set_error("layer norm: mean and rstd go together");
     if (!a.x) return set_error("null argument");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (n->type == GNNX_F32) run_forward<float>(a, s);
-    else if (n->type == GNNX_BF16) run_forward<bf16_t>(a, s);
-    else run_forward<f16_t>(a, s);
+    if (n->type == GNNX_F32) a.d ? run_forward<float, true>(a, s) : run_forward<float, false>(a, s);
+    else if (n->type == GNNX_BF16) a.d ? run_forward<bf16_t, true>(a, s) : run_forward<bf16_t, false>(a, s);
+    else a.d ? run_forward<f16_t, true>(a, s) : run_forward<f16_t, false>(a, s);
     return launched("gnnx_layer_norm_forward");
 }
 
@@ -148,7 +169,7 @@ extern "C" int gnnx_dropout(int32_t type, int64_t rows, int64_t cols, const void
     if (rows == 0 || cols == 0) return 0;
     if (!x || !y) return set_error("null argument");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const dim3 grid(grid_of(rows * ((cols + 3) / 4), 256)), block(256);
+    const dim3 grid(grid_of(rows * ((cols + 3) / 4), 256, 256)), block(256);
     if (type == GNNX_F32) hipLaunchKernelGGL((k_dropout<float>), grid, block, 0, s, rows, cols, x_stride, static_cast<const float*>(x), static_cast<float*>(y), d);
     else if (type == GNNX_BF16) hipLaunchKernelGGL((k_dropout<bf16_t>), grid, block, 0, s, rows, cols, x_stride, static_cast<const bf16_t*>(x), static_cast<bf16_t*>(y), d);
     else hipLaunchKernelGGL((k_dropout<f16_t>), grid, block, 0, s, rows, cols, x_stride, static_cast<const f16_t*>(x), static_cast<f16_t*>(y), d);
