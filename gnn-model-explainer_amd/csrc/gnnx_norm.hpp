@@ -159,7 +159,8 @@ __device__ __forceinline__ void drop_piece(const DropArgs& d, const DropKey& key
         const int sh = (int)(c & 3);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const uint32_t lo = sh & 1 ? w[j + 1] : w[j], hi = sh & 1 ? w[j + 3] : w[j + 2];
+            const uint32_t w0 = w[j], w1 = w[j + 1], w2 = w[j + 2], w3 = w[j + 3];      // (values: a choice between the elements would index memory)
+            const uint32_t lo = sh & 1 ? w1 : w0, hi = sh & 1 ? w3 : w2;
             v[j] = dropped(d, sh & 2 ? hi : lo, v[j]);
         }
     }
@@ -408,17 +409,150 @@ __global__ __launch_bounds__(256) void k_norm_backward_cols(NormArgs a) {
     if (wave < 2 && c < a.cols) a.part[(part * 2 + wave) * a.cols + c] = (sums[wave][0][lane] + sums[wave][1][lane]) + (sums[wave][2][lane] + sums[wave][3][lane]);
 }
 
-// The partial sums of a column, in part order.
+// The backward pass of rows in registers: one pass over x, dy (and dd), dx out.  COLS: a workgroup walks rows a grid apart and keeps its share of dw and db in
+// registers; at the end the lanes that hold the same column add up (lane swaps, then LDS across the waves) and the workgroup leaves one partial row of each.
+template <class T, int TPR, int K, bool DROP, bool COLS>
+__global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs a) {
+    constexpr int V = Piece<T>::V, RPB = norm_threads<TPR>() / TPR;
+    __shared__ float part[2][TPR > 64 ? TPR / 64 : 1][2];
+    const int l = threadIdx.x % TPR;
+    const float inv = 1.0f / (float)a.cols;
+    const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
+    Slot at[K];
+    float sw[K][V], sb[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        at[k] = slot_at<V>((k * TPR + l) * V, a.cols);
+#pragma unroll
+        for (int j = 0; j < V; ++j) sw[k][j] = sb[k][j] = 0.0f;
+    }
+    int turn = 0;
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB, turn ^= 1) {
+        const bool live = r0 + threadIdx.x / TPR < a.rows;
+        const int64_t r = live ? r0 + threadIdx.x / TPR : a.rows - 1;
+        const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
+        Piece<T> q[K];
+        float g[K][V], s[2] = {0.0f, 0.0f};
+        const float mean = a.mean[r], rstd = a.rstd[r];
+#pragma unroll
+        for (int k = 0; k < K; ++k) q[k] = load_piece(x + at[k].c);
+        if (a.dy) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const Piece<T> p = load_piece(static_cast<const T*>(a.dy) + r * a.dy_stride + at[k].c);
+#pragma unroll
+                for (int j = 0; j < V; ++j) g[k][j] = p.at(j);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < V; ++j) g[k][j] = 0.0f;
+        }
+        if (DROP) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const Piece<T> p = load_piece(static_cast<const T*>(a.dd) + r * a.dd_stride + at[k].c);
+                float d[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) d[j] = p.at(j);
+                drop_piece<T>(a.drop, key, r, at[k].c, a.cols, d);
+#pragma unroll
+                for (int j = 0; j < V; ++j) g[k][j] += d[j];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float p[V];
+            if (a.w) load_params<T>(p, a.w, a.w_is_f32, at[k].c);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float xhat = (floored(q[k].at(j), a.relu_floor) - mean) * rstd;
+                const bool mine = (2 * k + 1 < K || j >= at[k].skip) && (RPB == 1 || live);
+                if (COLS) {
+                    sb[k][j] += mine ? g[k][j] : 0.0f;
+                    sw[k][j] += mine ? g[k][j] * xhat : 0.0f;
+                }
+                if (a.w) g[k][j] *= p[j];
+                s[0] += mine ? g[k][j] : 0.0f;
+                s[1] += mine ? g[k][j] * xhat : 0.0f;
+            }
+        }
+        if (!a.dx) continue;
+        row_totals<TPR>(s, part[turn]);
+        const float c1 = s[0] * inv, c2 = s[1] * inv;
+        if (!live) continue;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (at[k].skip < V) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float xv = q[k].at(j), xhat = (floored(xv, a.relu_floor) - mean) * rstd, d = rstd * (g[k][j] - c1 - xhat * c2);
+                    g[k][j] = a.relu && xv <= 0.0f ? 0.0f : d;
+                }
+                store_piece(static_cast<T*>(a.dx) + r * a.cols + at[k].c, g[k]);
+            }
+        }
+    }
+    if constexpr (COLS) {
+        if constexpr (TPR < 64) {
+#pragma unroll
+            for (int o = TPR; o < 64; o <<= 1)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    sw[0][j] += __shfl_xor(sw[0][j], o);
+                    sb[0][j] += __shfl_xor(sb[0][j], o);
+                }
+        }
+        const int wave = threadIdx.x >> 6;
+        __shared__ float lds[RPB > 1 ? 3 : 1][2][RPB > 1 ? V : 1][RPB > 1 ? TPR : 1];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if constexpr (RPB > 1) {
+                if (k) __syncthreads();
+                if (wave && (threadIdx.x & 63) < TPR)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        lds[wave - 1][0][j][l] = sw[k][j];
+                        lds[wave - 1][1][j][l] = sb[k][j];
+                    }
+                __syncthreads();
+                if (threadIdx.x >= TPR) continue;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    sw[k][j] = (sw[k][j] + lds[0][0][j][l]) + (lds[1][0][j][l] + lds[2][0][j][l]);
+                    sb[k][j] = (sb[k][j] + lds[0][1][j][l]) + (lds[1][1][j][l] + lds[2][1][j][l]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (j >= at[k].skip) {
+                    a.part[(int64_t)blockIdx.x * 2 * a.cols + at[k].c + j] = sw[k][j];
+                    a.part[((int64_t)blockIdx.x * 2 + 1) * a.cols + at[k].c + j] = sb[k][j];
+                }
+        }
+    }
+}
+
+// The partial sums of a column: 32 columns and 32 parts at a time per workgroup, each of the 32 sums in part order, then the 32 in order.
 template <class T>
-__global__ __launch_bounds__(256) void k_norm_join(NormArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;      // dw's columns, then db's
-    if (i >= 2 * a.cols) return;
-    const bool is_b = i >= a.cols;
-    const int64_t c = is_b ? i - a.cols : i;
-    void* out = is_b ? a.db : a.dw;
-    if (!out) return;
+__global__ __launch_bounds__(1024) void k_norm_join(NormArgs a) {
+    __shared__ float sums[32][33];
+    const int64_t i = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31), n = 2 * a.cols;      // dw's columns, then db's
     float s = 0.0f;
-    for (int p = 0; p < a.parts; ++p) s += a.part[((int64_t)p * 2 + is_b) * a.cols + c];
+    if (i < n) {
+#pragma unroll 8
+        for (int p = threadIdx.x >> 5; p < a.parts; p += 32) s += a.part[(int64_t)p * n + i];
+    }
+    sums[threadIdx.x >> 5][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (threadIdx.x >= 32 || i >= n) return;
+    s = 0.0f;
+#pragma unroll
+    for (int p = 0; p < 32; ++p) s += sums[p][threadIdx.x];
+    void* out = i >= a.cols ? a.db : a.dw;
+    const int64_t c = i >= a.cols ? i - a.cols : i;
+    if (!out) return;
     if (a.w_is_f32) static_cast<float*>(out)[c] = s;
     else static_cast<T*>(out)[c] = (T)s;
 }

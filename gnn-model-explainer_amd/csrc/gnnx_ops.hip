@@ -75,10 +75,29 @@ const char* norm_args(const gnnx_norm* n, NormArgs* a) {
     return nullptr;
 }
 
-int col_parts(int64_t rows, int64_t cols) {
-    const int64_t tiles = (cols + 63) / 64;
-    int64_t parts = 2048 / tiles;
-    if (parts > (rows + 15) / 16) parts = (rows + 15) / 16;
+// How the backward pass of a row is shared out: lanes per row and pieces per lane; lanes == 0: the row does not fit registers (or is shorter than a piece).
+struct RowShape { int lanes, pieces; };
+RowShape backward_shape(int32_t type, int64_t cols) {
+    const int64_t v = type == GNNX_F32 ? 4 : 8, pieces = (cols + v - 1) / v;
+    if (cols < v || pieces > 2048) return {0, 0};
+    for (int lanes = 1; lanes <= 64; lanes *= 2)
+        if (pieces <= lanes) return {lanes, 1};
+    return pieces <= 128 ? RowShape{64, 2} : pieces <= 256 ? RowShape{64, 4} : pieces <= 512 ? RowShape{256, 2} : pieces <= 1024 ? RowShape{256, 4} : RowShape{512, 4};
+}
+
+// Partial rows of dw and db: one per workgroup of k_norm_backward, or per slice of the rows of k_norm_backward_cols.
+int col_parts(int32_t type, int64_t rows, int64_t cols) {
+    const RowShape sh = backward_shape(type, cols);
+    int64_t parts;
+    if (sh.lanes) {
+        const int64_t per = sh.lanes <= 64 ? 256 / sh.lanes : 1, groups = (rows + per - 1) / per;
+        parts = groups / 2;
+        if (parts > 1024) parts = 1024;
+    } else {
+        const int64_t tiles = (cols + 63) / 64;
+        parts = 2048 / tiles;
+        if (parts > (rows + 15) / 16) parts = (rows + 15) / 16;
+    }
     return (int)(parts < 1 ? 1 : parts);
 }
 
@@ -109,13 +128,33 @@ void run_forward(const NormArgs& a, hipStream_t s) {
     else hipLaunchKernelGGL((k_norm_forward_long<T, DROP>), dim3(grid_of(a.rows, 1, 1024)), dim3(1024), 0, s, a);
 }
 
+template <class T, int TPR, int K, bool DROP>
+void backward_rows(const NormArgs& a, hipStream_t s) {
+    constexpr int NT = norm_threads<TPR>();
+    if (a.parts) hipLaunchKernelGGL((k_norm_backward<T, TPR, K, DROP, true>), dim3((unsigned)a.parts), dim3(NT), 0, s, a);
+    else if (a.rows) hipLaunchKernelGGL((k_norm_backward<T, TPR, K, DROP, false>), dim3(grid_of(a.rows, NT / TPR, NT)), dim3(NT), 0, s, a);
+}
+
 template <class T, bool DROP>
-void run_backward(const NormArgs& a, hipStream_t s) {
-    if (a.dx && a.rows) hipLaunchKernelGGL((k_norm_backward_rows<T, DROP>), dim3(grid_of(a.rows, 4, 256)), dim3(256), 0, s, a);
-    if (!a.dw && !a.db) return;
-    const unsigned tiles = (unsigned)((a.cols + 63) / 64);
-    hipLaunchKernelGGL((k_norm_backward_cols<T, DROP>), dim3(tiles * (unsigned)a.parts), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((k_norm_join<T>), dim3((unsigned)((2 * a.cols + 255) / 256)), dim3(256), 0, s, a);
+void run_backward(const NormArgs& a, RowShape sh, hipStream_t s) {
+    switch (sh.lanes * 8 + sh.pieces) {
+        case 1 * 8 + 1: backward_rows<T, 1, 1, DROP>(a, s); break;
+        case 2 * 8 + 1: backward_rows<T, 2, 1, DROP>(a, s); break;
+        case 4 * 8 + 1: backward_rows<T, 4, 1, DROP>(a, s); break;
+        case 8 * 8 + 1: backward_rows<T, 8, 1, DROP>(a, s); break;
+        case 16 * 8 + 1: backward_rows<T, 16, 1, DROP>(a, s); break;
+        case 32 * 8 + 1: backward_rows<T, 32, 1, DROP>(a, s); break;
+        case 64 * 8 + 1: backward_rows<T, 64, 1, DROP>(a, s); break;
+        case 64 * 8 + 2: backward_rows<T, 64, 2, DROP>(a, s); break;
+        case 64 * 8 + 4: backward_rows<T, 64, 4, DROP>(a, s); break;
+        case 256 * 8 + 2: backward_rows<T, 256, 2, DROP>(a, s); break;
+        case 256 * 8 + 4: backward_rows<T, 256, 4, DROP>(a, s); break;
+        case 512 * 8 + 4: backward_rows<T, 512, 4, DROP>(a, s); break;
+        default:
+            if (a.dx && a.rows) hipLaunchKernelGGL((k_norm_backward_rows<T, DROP>), dim3(grid_of(a.rows, 4, 256)), dim3(256), 0, s, a);
+            if (a.parts) hipLaunchKernelGGL((k_norm_backward_cols<T, DROP>), dim3((unsigned)((a.cols + 63) / 64) * (unsigned)a.parts), dim3(256), 0, s, a);
+    }
+    if (a.parts) hipLaunchKernelGGL((k_norm_join<T>), dim3((unsigned)((2 * a.cols + 31) / 32)), dim3(1024), 0, s, a);
 }
 
 }  // namespace
@@ -136,9 +175,9 @@ extern "C" int gnnx_layer_norm_forward(const gnnx_norm* n, const gnnx_drop* drop
     return launched("gnnx_layer_norm_forward");
 }
 
-extern "C" size_t gnnx_layer_norm_workspace_bytes(int32_t, int64_t rows, int64_t cols) {
+extern "C" size_t gnnx_layer_norm_workspace_bytes(int32_t type, int64_t rows, int64_t cols) {
     if (rows < 0 || cols < 1) return 0;
-    return (size_t)col_parts(rows, cols) * 2 * (size_t)cols * sizeof(float);
+    return (size_t)col_parts(type, rows, cols) * 2 * (size_t)cols * sizeof(float);
 }
 
 extern "C" int gnnx_layer_norm_backward(const gnnx_norm* n, const gnnx_drop* drop, void* workspace, size_t workspace_bytes, void* stream) {
@@ -151,12 +190,13 @@ extern "C" int gnnx_layer_norm_backward(const gnnx_norm* n, const gnnx_drop* dro
     if (a.dw || a.db) {
         if (!workspace || workspace_bytes < gnnx_layer_norm_workspace_bytes(n->type, a.rows, a.cols)) return set_error("workspace too small");
         a.part = static_cast<float*>(workspace);
-        a.parts = col_parts(a.rows, a.cols);
+        a.parts = col_parts(n->type, a.rows, a.cols);
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (n->type == GNNX_F32) a.dd ? run_backward<float, true>(a, s) : run_backward<float, false>(a, s);
-    else if (n->type == GNNX_BF16) a.dd ? run_backward<bf16_t, true>(a, s) : run_backward<bf16_t, false>(a, s);
-    else a.dd ? run_backward<f16_t, true>(a, s) : run_backward<f16_t, false>(a, s);
+    const RowShape sh = backward_shape(n->type, a.cols);
+    if (n->type == GNNX_F32) a.dd ? run_backward<float, true>(a, sh, s) : run_backward<float, false>(a, sh, s);
+    else if (n->type == GNNX_BF16) a.dd ? run_backward<bf16_t, true>(a, sh, s) : run_backward<bf16_t, false>(a, sh, s);
+    else a.dd ? run_backward<f16_t, true>(a, sh, s) : run_backward<f16_t, false>(a, sh, s);
     return launched("gnnx_layer_norm_backward");
 }
 
