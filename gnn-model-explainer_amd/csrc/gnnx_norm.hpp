@@ -30,11 +30,14 @@ struct NormArgs {
     const void *x, *w, *b, *dy, *dd;
     void *y, *d, *dx, *dw, *db;
     float *mean, *rstd;
-    float eps, relu_floor;   // v = x < relu_floor ? relu_floor : x (0, or -inf without ReLU; NaN stays NaN)
-    int32_t relu;
+    float eps;
+    float relu_floor;        // v = maximum(x, relu_floor): 0, or -inf without ReLU
+    float relu_stop;         // dx = 0 where x <= relu_stop: 0, or NaN (never) without ReLU
     int32_t w_is_f32;        // type of w, b, dw, db: 1 fp32, 0 the type of x
-    float* part;             // [parts][2][cols] partial column sums of the backward pass
+    float* part;             // [parts][2][cols] partial sums of dw and db
     int32_t parts;
+    float* chunk;            // long rows: [rows][chunks][2] partial sums of the chunks of a row
+    int32_t chunks;
     DropArgs drop;
 };
 
@@ -70,7 +73,7 @@ __device__ __forceinline__ float dropped(const DropArgs& a, uint32_t word, float
     return word > a.last_dropped || !a.on ? v * a.scale : 0.0f;
 }
 
-__device__ __forceinline__ float floored(float v, float floor) { return v < floor ? floor : v; }      // ReLU (floor 0) or nothing (floor -inf); NaN stays
+__device__ __forceinline__ float floored(float v, float floor) { return __builtin_elementwise_maximum(v, floor); }      // ReLU or nothing; NaN stays NaN
 
 template <class T>
 __device__ __forceinline__ float param_at(const void* p, int32_t is_f32, int64_t c) {
@@ -166,13 +169,40 @@ __device__ __forceinline__ void drop_piece(const DropArgs& d, const DropKey& key
     }
 }
 
-// Sums over the TPR lanes that share a row, in every one of them; beyond a wave through `part` (one float per wave and sum).
+// all ones in the bits of a piece's elements that count (all but the first `skip`)
+template <class T>
+__device__ __forceinline__ u32x4 piece_mask(int skip) {
+    u32x4 m;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) m[j] = j >= skip ? ~0u : 0u;
+        else m[j] = (2 * j >= skip ? 0xffffu : 0u) | (2 * j + 1 >= skip ? 0xffff0000u : 0u);
+    }
+    return m;
+}
+
+// v + v of lane ^ O (O = 1, 2), of the lane mirrored in its 8 (O = 4) or 16 (O = 8) lanes - the same sum once the smaller groups hold theirs -, of lane ^ O
+template <int O>
+__device__ __forceinline__ float lane_pair_sum(float v) {
+    constexpr int ctrl = O == 1 ? 0xB1 : O == 2 ? 0x4E : O == 4 ? 0x141 : 0x140;
+    if constexpr (O > 8) return v + __shfl_xor(v, O);
+    else return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, true));
+}
+template <int TPR>
+__device__ __forceinline__ float lanes_total(float v) {
+    if constexpr (TPR > 1) v = lane_pair_sum<1>(v);
+    if constexpr (TPR > 2) v = lane_pair_sum<2>(v);
+    if constexpr (TPR > 4) v = lane_pair_sum<4>(v);
+    if constexpr (TPR > 8) v = lane_pair_sum<8>(v);
+    if constexpr (TPR > 16) v = lane_pair_sum<16>(v);
+    if constexpr (TPR > 32) v = lane_pair_sum<32>(v);
+    return v;
+}
+// Sums over the TPR lanes that share a row, in every one of them; beyond a wave through `part` (one float per wave and sum; two calls in a row need two).
 template <int TPR, int N>
 __device__ __forceinline__ void row_totals(float (&v)[N], float (*part)[N]) {
 #pragma unroll
-    for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1)
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
+    for (int i = 0; i < N; ++i) v[i] = lanes_total<(TPR < 64 ? TPR : 64)>(v[i]);
     if constexpr (TPR > 64) {
         constexpr int W = TPR / 64;
         if ((threadIdx.x & 63) == 0)
@@ -214,6 +244,32 @@ __device__ __forceinline__ void norm_outputs(const NormArgs& a, const DropKey& k
 template <int TPR>
 constexpr int norm_threads() { return TPR <= 64 ? 256 : TPR; }
 
+// sum of a lane's K pieces (first the mean's), and of their squared distances from `mean`: the elements that another piece has as well are left out
+template <class T, int K>
+__device__ __forceinline__ float pieces_sum(const Piece<T> (&q)[K], const Slot (&at)[K], float floor) {
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        Piece<T> p = q[k];
+        if (2 * k + 1 >= K) p.w &= piece_mask<T>(at[k].skip);      // (more than half of the K rounds are full: the launch's choice of K)
+#pragma unroll
+        for (int j = 0; j < Piece<T>::V; ++j) s += floored(p.at(j), floor);
+    }
+    return s;
+}
+template <class T, int K>
+__device__ __forceinline__ float pieces_squares(const Piece<T> (&q)[K], const Slot (&at)[K], float floor, float mean) {
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < Piece<T>::V; ++j) {
+            const float v = floored(q[k].at(j), floor) - mean;
+            s += 2 * k + 1 < K || j >= at[k].skip ? v * v : 0.0f;
+        }
+    return s;
+}
+
 template <class T, int TPR, int K, bool DROP>
 __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a) {
     constexpr int V = Piece<T>::V, RPB = norm_threads<TPR>() / TPR;
@@ -227,29 +283,15 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
         const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
         Piece<T> q[K];                             // as stored: widened again in each pass, half the registers for 16-bit types
         Slot at[K];
-        float s[1] = {0.0f};
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             at[k] = slot_at<V>((k * TPR + l) * V, a.cols);
             q[k] = load_piece(x + at[k].c);
         }
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float v = floored(q[k].at(j), a.relu_floor);
-                s[0] += 2 * k + 1 < K || j >= at[k].skip ? v : 0.0f;      // (more than half of the K rounds are full: run_forward)
-            }
+        float s[1] = {pieces_sum(q, at, a.relu_floor)};
         row_totals<TPR>(s, part[0]);
         const float mean = s[0] * inv;
-        s[0] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float v = floored(q[k].at(j), a.relu_floor) - mean;
-                s[0] += 2 * k + 1 < K || j >= at[k].skip ? v * v : 0.0f;
-            }
+        s[0] = pieces_squares(q, at, a.relu_floor, mean);
         row_totals<TPR>(s, part[1]);
         const float rstd = 1.0f / sqrtf(s[0] * inv + a.eps);
         if (!live) continue;
@@ -258,59 +300,109 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
             a.rstd[r] = rstd;
         }
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
+        for (int k = 0; k < K; ++k)
             if (at[k].skip < V) {
                 float v[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[j] = (floored(q[k].at(j), a.relu_floor) - mean) * rstd;
                 norm_outputs<T, DROP>(a, key, r, at[k].c, v);
             }
+    }
+}
+
+// ---- rows too long for a workgroup's registers: cut into chunks of CHUNK_LANES x CHUNK_PIECES pieces, a workgroup each, in two launches ----
+constexpr int CHUNK_LANES = 256, CHUNK_PIECES = 4;
+template <class T>
+constexpr int chunk_cols() { return CHUNK_LANES * CHUNK_PIECES * Piece<T>::V; }
+// the slots of a lane in chunk `ch`; every chunk but a row's last is full
+template <class T>
+__device__ __forceinline__ void chunk_slots(Slot (&at)[CHUNK_PIECES], int ch, int64_t cols) {
+#pragma unroll
+    for (int k = 0; k < CHUNK_PIECES; ++k)
+        at[k] = slot_at<Piece<T>::V>((int64_t)ch * chunk_cols<T>() + (k * CHUNK_LANES + (int)threadIdx.x) * Piece<T>::V, cols);
+}
+
+// First launch of the forward pass: the chunk's mean and its sum of squared distances from that mean.
+template <class T>
+__global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_stats(NormArgs a) {
+    __shared__ float part[2][CHUNK_LANES / 64][1];
+    const int64_t units = a.rows * a.chunks;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int64_t r = u / a.chunks;
+        const int ch = (int)(u % a.chunks);
+        Slot at[CHUNK_PIECES];
+        Piece<T> q[CHUNK_PIECES];
+        chunk_slots<T>(at, ch, a.cols);
+#pragma unroll
+        for (int k = 0; k < CHUNK_PIECES; ++k) q[k] = load_piece(static_cast<const T*>(a.x) + r * a.x_stride + at[k].c);
+        float s[1] = {0.0f};
+#pragma unroll
+        for (int k = 0; k < CHUNK_PIECES; ++k) {
+            Piece<T> p = q[k];
+            p.w &= piece_mask<T>(at[k].skip);
+#pragma unroll
+            for (int j = 0; j < Piece<T>::V; ++j) s[0] += floored(p.at(j), a.relu_floor);
+        }
+        row_totals<CHUNK_LANES>(s, part[0]);
+        const int64_t left = a.cols - (int64_t)ch * chunk_cols<T>();
+        const float mean = s[0] / (float)(left < chunk_cols<T>() ? left : chunk_cols<T>());
+        s[0] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < CHUNK_PIECES; ++k)
+#pragma unroll
+            for (int j = 0; j < Piece<T>::V; ++j) {
+                const float v = floored(q[k].at(j), a.relu_floor) - mean;
+                s[0] += j >= at[k].skip ? v * v : 0.0f;
+            }
+        row_totals<CHUNK_LANES>(s, part[1]);
+        if (threadIdx.x == 0) {
+            a.chunk[2 * u] = mean;
+            a.chunk[2 * u + 1] = s[0];
         }
     }
 }
 
-// Rows too long for registers: one workgroup per row, the row read again for each of the three passes (mean, squared distance from it, output).
+// Second launch: the row's statistics from its chunks' - sum of squares = sum of the chunks' + their sizes times the squared distance of their means from the
+// row's - in every workgroup alike, then the chunk's outputs.
 template <class T, bool DROP>
-__global__ __launch_bounds__(1024) void k_norm_forward_long(NormArgs a) {
-    constexpr int V = Piece<T>::V;
-    __shared__ float part[2][16][1];
-    const float inv = 1.0f / (float)a.cols;
+__global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_outputs(NormArgs a) {
     const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
-        float s[1] = {0.0f};
-        for (int64_t c = (int64_t)threadIdx.x * V; c < a.cols; c += 1024 * V) {
-            const Slot t = slot_at<V>(c, a.cols);
-            const Piece<T> q = load_piece(x + t.c);
+    const int64_t units = a.rows * a.chunks;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int64_t r = u / a.chunks;
+        const int ch = (int)(u % a.chunks);
+        Slot at[CHUNK_PIECES];
+        Piece<T> q[CHUNK_PIECES];
+        chunk_slots<T>(at, ch, a.cols);
 #pragma unroll
-            for (int j = 0; j < V; ++j) s[0] += j >= t.skip ? floored(q.at(j), a.relu_floor) : 0.0f;
+        for (int k = 0; k < CHUNK_PIECES; ++k) q[k] = load_piece(static_cast<const T*>(a.x) + r * a.x_stride + at[k].c);
+        const float* st = a.chunk + 2 * r * a.chunks;
+        const int lane = threadIdx.x & 63;
+        float s = 0.0f;
+        for (int i = lane; i < a.chunks; i += 64) {
+            const int64_t left = a.cols - (int64_t)i * chunk_cols<T>();
+            s += st[2 * i] * (float)(left < chunk_cols<T>() ? left : chunk_cols<T>());
         }
-        row_totals<1024>(s, part[0]);
-        const float mean = s[0] * inv;
-        s[0] = 0.0f;
-        for (int64_t c = (int64_t)threadIdx.x * V; c < a.cols; c += 1024 * V) {
-            const Slot t = slot_at<V>(c, a.cols);
-            const Piece<T> q = load_piece(x + t.c);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float v = floored(q.at(j), a.relu_floor) - mean;
-                s[0] += j >= t.skip ? v * v : 0.0f;
-            }
+        const float mean = lanes_total<64>(s) / (float)a.cols;
+        s = 0.0f;
+        for (int i = lane; i < a.chunks; i += 64) {
+            const int64_t left = a.cols - (int64_t)i * chunk_cols<T>();
+            const float d = st[2 * i] - mean;
+            s += st[2 * i + 1] + d * d * (float)(left < chunk_cols<T>() ? left : chunk_cols<T>());
         }
-        row_totals<1024>(s, part[1]);
-        const float rstd = 1.0f / sqrtf(s[0] * inv + a.eps);
-        if (threadIdx.x == 0 && a.mean) {
+        const float rstd = 1.0f / sqrtf(lanes_total<64>(s) / (float)a.cols + a.eps);
+        if (ch == 0 && threadIdx.x == 0 && a.mean) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
         }
-        for (int64_t c = (int64_t)threadIdx.x * V; c < a.cols; c += 1024 * V) {
-            const Slot t = slot_at<V>(c, a.cols);
-            const Piece<T> q = load_piece(x + t.c);
-            float v[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = (floored(q.at(j), a.relu_floor) - mean) * rstd;
-            norm_outputs<T, DROP>(a, key, r, t.c, v);
-        }
+        for (int k = 0; k < CHUNK_PIECES; ++k)
+            if (at[k].skip < Piece<T>::V) {
+                float v[Piece<T>::V];
+#pragma unroll
+                for (int j = 0; j < Piece<T>::V; ++j) v[j] = (floored(q[k].at(j), a.relu_floor) - mean) * rstd;
+                norm_outputs<T, DROP>(a, key, r, at[k].c, v);
+            }
     }
 }
 
@@ -344,73 +436,86 @@ __global__ __launch_bounds__(256) void k_norm_forward_narrow(NormArgs a) {
     }
 }
 
-__device__ __forceinline__ float wave_total(float v) {
+// ---- backward ----
+// What a lane holds of one row: its pieces of x, dy and dd as stored.  Where a piece was moved back, dy and dd are blanked in the elements that count elsewhere:
+// they then add nothing to any sum, and only the elements that count are stored.
+template <class T, int K, bool DROP>
+struct RowPieces {
+    Piece<T> x[K], dy[K], dd[DROP ? K : 1];
+    float mean, rstd;
+    __device__ __forceinline__ void load(const NormArgs& a, const Slot (&at)[K], int64_t r, bool live) {
+        const T* xr = static_cast<const T*>(a.x) + r * a.x_stride;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-    return v;
-}
-
-// dL/dy at (r, c): the gradient of the kept output plus that of the dropped one
-template <class T, bool DROP>
-__device__ __forceinline__ float norm_dy(const NormArgs& a, const DropKey& key, int64_t r, int64_t c) {
-    float g = a.dy ? (float)static_cast<const T*>(a.dy)[r * a.dy_stride + c] : 0.0f;
-    if (DROP) g += dropped(a.drop, drop_words(a.drop, key, r, (uint32_t)(c >> 2)).w[c & 3], (float)static_cast<const T*>(a.dd)[r * a.dd_stride + c]);
-    return g;
-}
-
-template <class T, bool DROP>
-__global__ __launch_bounds__(256) void k_norm_backward_rows(NormArgs a) {
-    const int lane = threadIdx.x & 63;
-    const float inv = 1.0f / (float)a.cols;
-    const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * 4) {
-        const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
-        const float mean = a.mean[r], rstd = a.rstd[r];
-        float s1 = 0.0f, s2 = 0.0f;
-        for (int64_t c = lane; c < a.cols; c += 64) {
-            float v = (float)x[c], g = norm_dy<T, DROP>(a, key, r, c);
-            v = ((v < a.relu_floor ? a.relu_floor : v) - mean) * rstd;
-            if (a.w) g *= param_at<T>(a.w, a.w_is_f32, c);
-            s1 += g;
-            s2 += g * v;
+        for (int k = 0; k < K; ++k) x[k] = load_piece(xr + at[k].c);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (a.dy) dy[k] = load_piece(static_cast<const T*>(a.dy) + r * a.dy_stride + at[k].c);
+            else dy[k].w = (u32x4)0u;
+            if constexpr (DROP) dd[k] = load_piece(static_cast<const T*>(a.dd) + r * a.dd_stride + at[k].c);
         }
-        const float c1 = wave_total(s1) * inv, c2 = wave_total(s2) * inv;
-        for (int64_t c = lane; c < a.cols; c += 64) {
-            const float xv = (float)x[c];
-            float v = xv, g = norm_dy<T, DROP>(a, key, r, c);
-            v = ((v < a.relu_floor ? a.relu_floor : v) - mean) * rstd;
-            if (a.w) g *= param_at<T>(a.w, a.w_is_f32, c);
-            g = rstd * (g - c1 - v * c2);
-            static_cast<T*>(a.dx)[r * a.cols + c] = (T)(a.relu && xv <= 0.0f ? 0.0f : g);
+        mean = a.mean[r];
+        rstd = a.rstd[r];
+        if (!live) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                dy[k].w = (u32x4)0u;
+                if constexpr (DROP) dd[k].w = (u32x4)0u;
+            }
         }
+    }
+    // dL/dy of piece k
+    __device__ __forceinline__ void gradient(const NormArgs& a, const DropKey& key, const Slot& at, const u32x4& mask, int64_t r, int k, float* g) {
+        Piece<T> p = dy[k];
+        if (2 * k + 1 >= K) p.w &= mask;
+#pragma unroll
+        for (int j = 0; j < Piece<T>::V; ++j) g[j] = p.at(j);
+        if constexpr (DROP) {
+            Piece<T> e = dd[k];
+            if (2 * k + 1 >= K) e.w &= mask;
+            float d[Piece<T>::V];
+#pragma unroll
+            for (int j = 0; j < Piece<T>::V; ++j) d[j] = e.at(j);
+            drop_piece<T>(a.drop, key, r, at.c, a.cols, d);
+#pragma unroll
+            for (int j = 0; j < Piece<T>::V; ++j) g[j] += d[j];
+        }
+    }
+};
+
+// dx of one piece from g = dy w; a piece that was moved back stores its own elements only
+template <class T>
+__device__ __forceinline__ void store_dx(const NormArgs& a, const Piece<T>& x, const Slot& at, int64_t r, float mean, float rstd, float c1, float c2, const float* g) {
+    constexpr int V = Piece<T>::V;
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float xv = x.at(j), xhat = (floored(xv, a.relu_floor) - mean) * rstd, d = rstd * (g[j] - c1 - xhat * c2);
+        v[j] = xv <= a.relu_stop ? 0.0f : d;
+    }
+    T* out = static_cast<T*>(a.dx) + r * a.cols + at.c;
+    if (at.skip == 0) {
+        store_piece(out, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j >= at.skip) out[j] = (T)v[j];
     }
 }
 
-// Partial column sums: workgroup (column tile of 64, part) adds the rows r = 4 part + wave mod 4 parts; the four waves join in LDS.
-template <class T, bool DROP>
-__global__ __launch_bounds__(256) void k_norm_backward_cols(NormArgs a) {
-    __shared__ float sums[2][4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t tiles = (a.cols + 63) / 64;
-    const int64_t part = blockIdx.x / tiles, c = (blockIdx.x % tiles) * 64 + lane;
-    const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
-    float sw = 0.0f, sb = 0.0f;
-    if (c < a.cols)
-        for (int64_t r = part * 4 + wave; r < a.rows; r += (int64_t)a.parts * 4) {
-            float v = (float)(static_cast<const T*>(a.x)[r * a.x_stride + c]);
-            const float g = norm_dy<T, DROP>(a, key, r, c);
-            v = ((v < a.relu_floor ? a.relu_floor : v) - a.mean[r]) * a.rstd[r];
-            sw += g * v;
-            sb += g;
+// a lane's partial sums of dw and db, of the columns that count with it
+template <int V>
+__device__ __forceinline__ void store_cols(const NormArgs& a, int64_t part, const Slot& at, const float* sw, const float* sb) {
+    float* out = a.part + part * 2 * a.cols + at.c;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (j >= at.skip) {
+            out[j] = sw[j];
+            out[a.cols + j] = sb[j];
         }
-    sums[0][wave][lane] = sw;
-    sums[1][wave][lane] = sb;
-    __syncthreads();
-    if (wave < 2 && c < a.cols) a.part[(part * 2 + wave) * a.cols + c] = (sums[wave][0][lane] + sums[wave][1][lane]) + (sums[wave][2][lane] + sums[wave][3][lane]);
 }
 
 // The backward pass of rows in registers: one pass over x, dy (and dd), dx out.  COLS: a workgroup walks rows a grid apart and keeps its share of dw and db in
-// registers; at the end the lanes that hold the same column add up (lane swaps, then LDS across the waves) and the workgroup leaves one partial row of each.
+// registers; at the end the lanes that hold the same column add up (lane sums, then LDS across the waves) and the workgroup leaves one partial row of each.
 template <class T, int TPR, int K, bool DROP, bool COLS>
 __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs a) {
     constexpr int V = Piece<T>::V, RPB = norm_threads<TPR>() / TPR;
@@ -419,80 +524,64 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs 
     const float inv = 1.0f / (float)a.cols;
     const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
     Slot at[K];
+    u32x4 mask[K];
     float sw[K][V], sb[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         at[k] = slot_at<V>((k * TPR + l) * V, a.cols);
+        mask[k] = piece_mask<T>(at[k].skip);
 #pragma unroll
         for (int j = 0; j < V; ++j) sw[k][j] = sb[k][j] = 0.0f;
     }
     int turn = 0;
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB, turn ^= 1) {
-        const bool live = r0 + threadIdx.x / TPR < a.rows;
-        const int64_t r = live ? r0 + threadIdx.x / TPR : a.rows - 1;
-        const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
-        Piece<T> q[K];
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    int64_t r0 = (int64_t)blockIdx.x * RPB;
+    const auto row_of = [&](int64_t base, bool* live) {
+        const int64_t r = base + threadIdx.x / TPR;
+        *live = RPB == 1 || r < a.rows;
+        return *live ? r : a.rows - 1;
+    };
+    RowPieces<T, K, DROP> now, next;
+    bool live, next_live;
+    int64_t r, next_r;
+    if (r0 < a.rows) {
+        r = row_of(r0, &live);
+        now.load(a, at, r, live);
+    }
+    for (; r0 < a.rows; r0 += step, turn ^= 1) {
+        if (r0 + step < a.rows) {                  // the next row is on its way while this one is worked on
+            next_r = row_of(r0 + step, &next_live);
+            next.load(a, at, next_r, next_live);
+        }
         float g[K][V], s[2] = {0.0f, 0.0f};
-        const float mean = a.mean[r], rstd = a.rstd[r];
-#pragma unroll
-        for (int k = 0; k < K; ++k) q[k] = load_piece(x + at[k].c);
-        if (a.dy) {
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                const Piece<T> p = load_piece(static_cast<const T*>(a.dy) + r * a.dy_stride + at[k].c);
-#pragma unroll
-                for (int j = 0; j < V; ++j) g[k][j] = p.at(j);
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < K; ++k)
-#pragma unroll
-                for (int j = 0; j < V; ++j) g[k][j] = 0.0f;
-        }
-        if (DROP) {
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                const Piece<T> p = load_piece(static_cast<const T*>(a.dd) + r * a.dd_stride + at[k].c);
-                float d[V];
-#pragma unroll
-                for (int j = 0; j < V; ++j) d[j] = p.at(j);
-                drop_piece<T>(a.drop, key, r, at[k].c, a.cols, d);
-#pragma unroll
-                for (int j = 0; j < V; ++j) g[k][j] += d[j];
-            }
-        }
 #pragma unroll
         for (int k = 0; k < K; ++k) {
+            now.gradient(a, key, at[k], mask[k], r, k, g[k]);
             float p[V];
             if (a.w) load_params<T>(p, a.w, a.w_is_f32, at[k].c);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float xhat = (floored(q[k].at(j), a.relu_floor) - mean) * rstd;
-                const bool mine = (2 * k + 1 < K || j >= at[k].skip) && (RPB == 1 || live);
+                const float xhat = (floored(now.x[k].at(j), a.relu_floor) - now.mean) * now.rstd;
                 if (COLS) {
-                    sb[k][j] += mine ? g[k][j] : 0.0f;
-                    sw[k][j] += mine ? g[k][j] * xhat : 0.0f;
+                    sb[k][j] += g[k][j];
+                    sw[k][j] += g[k][j] * xhat;
                 }
                 if (a.w) g[k][j] *= p[j];
-                s[0] += mine ? g[k][j] : 0.0f;
-                s[1] += mine ? g[k][j] * xhat : 0.0f;
+                s[0] += g[k][j];
+                s[1] += g[k][j] * xhat;
             }
         }
-        if (!a.dx) continue;
-        row_totals<TPR>(s, part[turn]);
-        const float c1 = s[0] * inv, c2 = s[1] * inv;
-        if (!live) continue;
+        if (a.dx) {
+            row_totals<TPR>(s, part[turn]);
+            const float c1 = s[0] * inv, c2 = s[1] * inv;
+            if (live)
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            if (at[k].skip < V) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float xv = q[k].at(j), xhat = (floored(xv, a.relu_floor) - mean) * rstd, d = rstd * (g[k][j] - c1 - xhat * c2);
-                    g[k][j] = a.relu && xv <= 0.0f ? 0.0f : d;
-                }
-                store_piece(static_cast<T*>(a.dx) + r * a.cols + at[k].c, g[k]);
-            }
+                for (int k = 0; k < K; ++k)
+                    if (at[k].skip < V) store_dx(a, now.x[k], at[k], r, now.mean, now.rstd, c1, c2, g[k]);
         }
+        now = next;
+        r = next_r;
+        live = next_live;
     }
     if constexpr (COLS) {
         if constexpr (TPR < 64) {
@@ -524,13 +613,149 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs 
                     sb[k][j] = (sb[k][j] + lds[0][1][j][l]) + (lds[1][1][j][l] + lds[2][1][j][l]);
                 }
             }
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (j >= at[k].skip) {
-                    a.part[(int64_t)blockIdx.x * 2 * a.cols + at[k].c + j] = sw[k][j];
-                    a.part[((int64_t)blockIdx.x * 2 + 1) * a.cols + at[k].c + j] = sb[k][j];
-                }
+            store_cols<V>(a, blockIdx.x, at[k], sw[k], sb[k]);
         }
+    }
+}
+
+// Long rows, first launch of the backward pass: a chunk's sums of g and g xhat.
+template <class T, bool DROP>
+__global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_sums(NormArgs a) {
+    __shared__ float part[2][CHUNK_LANES / 64][2];
+    const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
+    const int64_t units = a.rows * a.chunks;
+    int turn = 0;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x, turn ^= 1) {
+        const int64_t r = u / a.chunks;
+        Slot at[CHUNK_PIECES];
+        chunk_slots<T>(at, (int)(u % a.chunks), a.cols);
+        RowPieces<T, CHUNK_PIECES, DROP> now;
+        now.load(a, at, r, true);
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < CHUNK_PIECES; ++k) {
+            const u32x4 mask = piece_mask<T>(at[k].skip);
+            now.dy[k].w &= mask;
+            if constexpr (DROP) now.dd[k].w &= mask;
+            float g[Piece<T>::V], p[Piece<T>::V];
+            now.gradient(a, key, at[k], mask, r, k, g);
+            if (a.w) load_params<T>(p, a.w, a.w_is_f32, at[k].c);
+#pragma unroll
+            for (int j = 0; j < Piece<T>::V; ++j) {
+                if (a.w) g[j] *= p[j];
+                s[0] += g[j];
+                s[1] += g[j] * ((floored(now.x[k].at(j), a.relu_floor) - now.mean) * now.rstd);
+            }
+        }
+        row_totals<CHUNK_LANES>(s, part[turn]);
+        if (threadIdx.x < 2) a.chunk[2 * u + threadIdx.x] = s[threadIdx.x];
+    }
+}
+
+// Second launch: workgroup (chunk, part) walks the rows part, part + parts, ...: dx of its chunk, and its share of dw and db.
+template <class T, bool DROP, bool COLS>
+__global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_backward(NormArgs a) {
+    constexpr int V = Piece<T>::V;
+    const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
+    const int ch = (int)(blockIdx.x % (unsigned)a.chunks), lane = threadIdx.x & 63;
+    const int64_t first = blockIdx.x / (unsigned)a.chunks, step = gridDim.x / (unsigned)a.chunks;
+    const float inv = 1.0f / (float)a.cols;
+    Slot at[CHUNK_PIECES];
+    chunk_slots<T>(at, ch, a.cols);
+    float sw[CHUNK_PIECES][V], sb[CHUNK_PIECES][V];
+#pragma unroll
+    for (int k = 0; k < CHUNK_PIECES; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) sw[k][j] = sb[k][j] = 0.0f;
+    for (int64_t r = first; r < a.rows; r += step) {
+        RowPieces<T, CHUNK_PIECES, DROP> now;
+        now.load(a, at, r, true);
+        float c1 = 0.0f, c2 = 0.0f;
+        if (a.dx) {
+            for (int i = lane; i < a.chunks; i += 64) {
+                c1 += a.chunk[2 * (r * a.chunks + i)];
+                c2 += a.chunk[2 * (r * a.chunks + i) + 1];
+            }
+            c1 = lanes_total<64>(c1) * inv;
+            c2 = lanes_total<64>(c2) * inv;
+        }
+#pragma unroll
+        for (int k = 0; k < CHUNK_PIECES; ++k) {
+            const u32x4 mask = piece_mask<T>(at[k].skip);
+            now.dy[k].w &= mask;
+            if constexpr (DROP) now.dd[k].w &= mask;
+            float g[V], p[V];
+            now.gradient(a, key, at[k], mask, r, k, g);
+            if (a.w) load_params<T>(p, a.w, a.w_is_f32, at[k].c);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (COLS) {
+                    sb[k][j] += g[j];
+                    sw[k][j] += g[j] * ((floored(now.x[k].at(j), a.relu_floor) - now.mean) * now.rstd);
+                }
+                if (a.w) g[j] *= p[j];
+            }
+            if (a.dx && at[k].skip < V) store_dx(a, now.x[k], at[k], r, now.mean, now.rstd, c1, c2, g);
+        }
+    }
+    if constexpr (COLS) {
+#pragma unroll
+        for (int k = 0; k < CHUNK_PIECES; ++k) store_cols<V>(a, first, at[k], sw[k], sb[k]);
+    }
+}
+
+// Rows shorter than one piece: one thread per row, its share of dw and db in registers (at most 7 columns), joined over the workgroup in LDS.
+template <class T, bool DROP>
+__global__ __launch_bounds__(256) void k_norm_backward_narrow(NormArgs a) {
+    constexpr int V = Piece<T>::V;
+    __shared__ float sums[4][2][V];
+    const float inv = 1.0f / (float)a.cols;
+    const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
+    float sw[V], sb[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) sw[c] = sb[c] = 0.0f;
+    for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < a.rows; r += (int64_t)gridDim.x * 256) {
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        float x[V], g[V], c1 = 0.0f, c2 = 0.0f;
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+            x[c] = g[c] = 0.0f;
+            if (c >= a.cols) continue;
+            x[c] = (float)static_cast<const T*>(a.x)[r * a.x_stride + c];
+            if (a.dy) g[c] = (float)static_cast<const T*>(a.dy)[r * a.dy_stride + c];
+            if (DROP)
+                g[c] += dropped(a.drop, drop_words(a.drop, key, r, (uint32_t)(c >> 2)).w[c & 3], (float)static_cast<const T*>(a.dd)[r * a.dd_stride + c]);
+            const float xhat = (floored(x[c], a.relu_floor) - mean) * rstd;
+            sb[c] += g[c];
+            sw[c] += g[c] * xhat;
+            if (a.w) g[c] *= param_at<T>(a.w, a.w_is_f32, c);
+            c1 += g[c];
+            c2 += g[c] * xhat;
+        }
+        c1 *= inv;
+        c2 *= inv;
+        if (!a.dx) continue;
+#pragma unroll
+        for (int c = 0; c < V; ++c)
+            if (c < a.cols) {
+                const float d = rstd * (g[c] - c1 - (floored(x[c], a.relu_floor) - mean) * rstd * c2);
+                static_cast<T*>(a.dx)[r * a.cols + c] = (T)(x[c] <= a.relu_stop ? 0.0f : d);
+            }
+    }
+    if (!a.parts) return;
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+        sw[c] = lanes_total<64>(sw[c]);
+        sb[c] = lanes_total<64>(sb[c]);
+        if ((threadIdx.x & 63) == 0) {
+            sums[threadIdx.x >> 6][0][c] = sw[c];
+            sums[threadIdx.x >> 6][1][c] = sb[c];
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < 2 * V) {
+        const int b = threadIdx.x / V, c = threadIdx.x % V;
+        if (c < a.cols) a.part[((int64_t)blockIdx.x * 2 + b) * a.cols + c] = (sums[0][b][c] + sums[1][b][c]) + (sums[2][b][c] + sums[3][b][c]);
     }
 }
 
@@ -557,22 +782,47 @@ __global__ __launch_bounds__(1024) void k_norm_join(NormArgs a) {
     else static_cast<T*>(out)[c] = (T)s;
 }
 
-// One thread per four columns of a row.
-template <class T>
-__global__ __launch_bounds__(256) void k_dropout(int64_t rows, int64_t cols, int64_t stride, const T* x, T* y, DropArgs d) {
-    const DropKey key = drop_key(d);
-    const int64_t blocks = (cols + 3) / 4;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * blocks; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / blocks, k = i % blocks;
-        Philox4 q = {};
-        if (d.on) q = drop_words(d, key, r, (uint32_t)k);
-        for (int j = 0; j < 4; ++j) {
-            const int64_t c = 4 * k + j;
-            if (c >= cols) break;
-            const float v = (float)x[r * stride + c];
-            y[r * cols + c] = (T)dropped(d, q.w[j], v);
-        }
+// ---- dropout alone ----
+struct DropoutArgs {
+    int64_t rows, cols, stride;
+    const void* x;
+    void* y;
+    uint32_t pieces, magic, shift;      // pieces of a row; n / pieces = (mulhi(n, magic) + n) >> shift for n < 2^32 (the sum in 33 bits)
+    DropArgs drop;
+};
+
+// One thread per piece of a row.  BIG: more pieces in all than 32 bits count.
+template <class T, bool BIG>
+__global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
+    constexpr int V = Piece<T>::V;
+    const DropKey key = drop_key(a.drop);
+    const int64_t n = a.rows * a.pieces;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        int64_t r;
+        if (BIG) r = i / a.pieces;
+        else r = (uint32_t)((((uint64_t)(uint32_t)i * a.magic >> 32) + (uint32_t)i) >> a.shift);
+        const Slot at = slot_at<V>((i - r * a.pieces) * V, a.cols);
+        const Piece<T> q = load_piece(static_cast<const T*>(a.x) + r * a.stride + at.c);
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = q.at(j);
+        if (a.drop.on) drop_piece<T>(a.drop, key, r, at.c, a.cols, v);
+        store_piece(static_cast<T*>(a.y) + r * a.cols + at.c, v);
     }
+}
+
+// Rows shorter than one piece: one thread per row.
+template <class T>
+__global__ __launch_bounds__(256) void k_dropout_narrow(DropoutArgs a) {
+    const DropKey key = drop_key(a.drop);
+    for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < a.rows; r += (int64_t)gridDim.x * 256)
+        for (int c = 0; c < a.cols; c += 4) {
+            const Philox4 q = drop_words(a.drop, key, r, (uint32_t)(c >> 2));
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j < a.cols)
+                    static_cast<T*>(a.y)[r * a.cols + c + j] = (T)dropped(a.drop, q.w[j], (float)static_cast<const T*>(a.x)[r * a.stride + c + j]);
+        }
 }
 
 }  // namespace gnnx

@@ -69,36 +69,59 @@ const char* norm_args(const gnnx_norm* n, NormArgs* a) {
     a->mean = n->mean;
     a->rstd = n->rstd;
     a->eps = n->eps;
-    a->relu = n->relu != 0;
     a->relu_floor = n->relu ? 0.0f : -std::numeric_limits<float>::infinity();
+    a->relu_stop = n->relu ? 0.0f : std::numeric_limits<float>::quiet_NaN();
     a->w_is_f32 = n->w_is_f32 != 0 || n->type == GNNX_F32;
     return nullptr;
 }
 
-// How the backward pass of a row is shared out: lanes per row and pieces per lane; lanes == 0: the row does not fit registers (or is shorter than a piece).
+// How a row is shared out: NARROW, shorter than a piece; LONG, cut into chunks; else `lanes` lanes with `pieces` pieces each.
+enum { NARROW = 0, LONG = -1 };
 struct RowShape { int lanes, pieces; };
-RowShape backward_shape(int32_t type, int64_t cols) {
-    const int64_t v = type == GNNX_F32 ? 4 : 8, pieces = (cols + v - 1) / v;
-    if (cols < v || pieces > 2048) return {0, 0};
+int64_t pieces_of(int32_t type, int64_t cols) { return type == GNNX_F32 ? (cols + 3) / 4 : (cols + 7) / 8; }
+// As few lanes as hold the row with one piece each up to a wave, then two to four pieces each before more waves join in.
+RowShape forward_shape(int32_t type, int64_t cols) {
+    const int64_t pieces = pieces_of(type, cols);
+    if (cols < (type == GNNX_F32 ? 4 : 8)) return {NARROW, 0};
     for (int lanes = 1; lanes <= 64; lanes *= 2)
         if (pieces <= lanes) return {lanes, 1};
-    return pieces <= 128 ? RowShape{64, 2} : pieces <= 256 ? RowShape{64, 4} : pieces <= 512 ? RowShape{256, 2} : pieces <= 1024 ? RowShape{256, 4} : RowShape{512, 4};
+    return pieces <= 128 ? RowShape{64, 2} : pieces <= 256 ? RowShape{64, 4} : pieces <= 512 ? RowShape{256, 2} : pieces <= 1024 ? RowShape{256, 4} :
+           pieces <= 2048 ? RowShape{1024, 2} : RowShape{LONG, 0};
+}
+RowShape backward_shape(int32_t type, int64_t cols) {
+    const int64_t pieces = pieces_of(type, cols);
+    if (cols < (type == GNNX_F32 ? 4 : 8)) return {NARROW, 0};
+    for (int lanes = 1; lanes <= 64; lanes *= 2)
+        if (pieces <= lanes) return {lanes, 1};
+    return pieces <= 128 ? RowShape{64, 2} : pieces <= 256 ? RowShape{256, 1} : pieces <= 512 ? RowShape{256, 2} : pieces <= 1024 ? RowShape{512, 2} : RowShape{LONG, 0};
+}
+int chunks_of(int32_t type, int64_t cols) {
+    const int64_t per = type == GNNX_F32 ? chunk_cols<float>() : chunk_cols<bf16_t>();
+    return (int)((cols + per - 1) / per);
 }
 
-// Partial rows of dw and db: one per workgroup of k_norm_backward, or per slice of the rows of k_norm_backward_cols.
+// Partial rows of dw and db: one per workgroup that walks rows.
 int col_parts(int32_t type, int64_t rows, int64_t cols) {
     const RowShape sh = backward_shape(type, cols);
     int64_t parts;
-    if (sh.lanes) {
-        const int64_t per = sh.lanes <= 64 ? 256 / sh.lanes : 1, groups = (rows + per - 1) / per;
+    if (sh.lanes == LONG) {
+        parts = 1024 / chunks_of(type, cols);
+        if (parts > rows / 2) parts = rows / 2;
+    } else {
+        const int64_t per = sh.lanes == NARROW ? 256 : sh.lanes <= 64 ? 256 / sh.lanes : 1, groups = (rows + per - 1) / per;
         parts = groups / 2;
         if (parts > 1024) parts = 1024;
-    } else {
-        const int64_t tiles = (cols + 63) / 64;
-        parts = 2048 / tiles;
-        if (parts > (rows + 15) / 16) parts = (rows + 15) / 16;
     }
     return (int)(parts < 1 ? 1 : parts);
+}
+
+size_t chunk_bytes(int32_t type, int64_t rows, int64_t cols) { return (size_t)rows * (size_t)chunks_of(type, cols) * 2 * sizeof(float); }
+
+size_t workspace_bytes_of(int32_t type, int64_t rows, int64_t cols, bool backward) {
+    size_t b = 0;
+    if ((backward ? backward_shape(type, cols) : forward_shape(type, cols)).lanes == LONG) b += chunk_bytes(type, rows, cols);
+    if (backward) b += (size_t)col_parts(type, rows, cols) * 2 * (size_t)cols * sizeof(float);
+    return b;
 }
 
 template <class T, int TPR, int K, bool DROP>
@@ -107,25 +130,27 @@ void forward_rows(const NormArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((k_norm_forward<T, TPR, K, DROP>), dim3(grid_of(a.rows, NT / TPR, NT)), dim3(NT), 0, s, a);
 }
 
-// The lanes of a row: as few as hold it with one piece each up to a wave, then two to eight pieces each before more waves join in.
 template <class T, bool DROP>
-void run_forward(const NormArgs& a, hipStream_t s) {
-    const int64_t pieces = (a.cols + Piece<T>::V - 1) / Piece<T>::V;
-    if (a.cols < Piece<T>::V) hipLaunchKernelGGL((k_norm_forward_narrow<T, DROP>), dim3(grid_of(a.rows, 256, 256)), dim3(256), 0, s, a);
-    else if (pieces <= 1) forward_rows<T, 1, 1, DROP>(a, s);
-    else if (pieces <= 2) forward_rows<T, 2, 1, DROP>(a, s);
-    else if (pieces <= 4) forward_rows<T, 4, 1, DROP>(a, s);
-    else if (pieces <= 8) forward_rows<T, 8, 1, DROP>(a, s);
-    else if (pieces <= 16) forward_rows<T, 16, 1, DROP>(a, s);
-    else if (pieces <= 32) forward_rows<T, 32, 1, DROP>(a, s);
-    else if (pieces <= 64) forward_rows<T, 64, 1, DROP>(a, s);
-    else if (pieces <= 128) forward_rows<T, 64, 2, DROP>(a, s);
-    else if (pieces <= 256) forward_rows<T, 64, 4, DROP>(a, s);
-    else if (pieces <= 512) forward_rows<T, 256, 2, DROP>(a, s);
-    else if (pieces <= 1024) forward_rows<T, 256, 4, DROP>(a, s);
-    else if (pieces <= 2048) forward_rows<T, 1024, 2, DROP>(a, s);
-    else if (pieces <= 4096) forward_rows<T, 1024, 4, DROP>(a, s);
-    else hipLaunchKernelGGL((k_norm_forward_long<T, DROP>), dim3(grid_of(a.rows, 1, 1024)), dim3(1024), 0, s, a);
+void run_forward(const NormArgs& a, RowShape sh, hipStream_t s) {
+    const unsigned units = grid_of(a.rows * a.chunks, 1, CHUNK_LANES);
+    switch (sh.lanes * 8 + sh.pieces) {
+        case 1 * 8 + 1: forward_rows<T, 1, 1, DROP>(a, s); break;
+        case 2 * 8 + 1: forward_rows<T, 2, 1, DROP>(a, s); break;
+        case 4 * 8 + 1: forward_rows<T, 4, 1, DROP>(a, s); break;
+        case 8 * 8 + 1: forward_rows<T, 8, 1, DROP>(a, s); break;
+        case 16 * 8 + 1: forward_rows<T, 16, 1, DROP>(a, s); break;
+        case 32 * 8 + 1: forward_rows<T, 32, 1, DROP>(a, s); break;
+        case 64 * 8 + 1: forward_rows<T, 64, 1, DROP>(a, s); break;
+        case 64 * 8 + 2: forward_rows<T, 64, 2, DROP>(a, s); break;
+        case 64 * 8 + 4: forward_rows<T, 64, 4, DROP>(a, s); break;
+        case 256 * 8 + 2: forward_rows<T, 256, 2, DROP>(a, s); break;
+        case 256 * 8 + 4: forward_rows<T, 256, 4, DROP>(a, s); break;
+        case 1024 * 8 + 2: forward_rows<T, 1024, 2, DROP>(a, s); break;
+        case NARROW: hipLaunchKernelGGL((k_norm_forward_narrow<T, DROP>), dim3(grid_of(a.rows, 256, 256)), dim3(256), 0, s, a); break;
+        default:
+            hipLaunchKernelGGL((k_norm_chunk_stats<T>), dim3(units), dim3(CHUNK_LANES), 0, s, a);
+            hipLaunchKernelGGL((k_norm_chunk_outputs<T, DROP>), dim3(units), dim3(CHUNK_LANES), 0, s, a);
+    }
 }
 
 template <class T, int TPR, int K, bool DROP>
@@ -146,20 +171,27 @@ void run_backward(const NormArgs& a, RowShape sh, hipStream_t s) {
         case 32 * 8 + 1: backward_rows<T, 32, 1, DROP>(a, s); break;
         case 64 * 8 + 1: backward_rows<T, 64, 1, DROP>(a, s); break;
         case 64 * 8 + 2: backward_rows<T, 64, 2, DROP>(a, s); break;
-        case 64 * 8 + 4: backward_rows<T, 64, 4, DROP>(a, s); break;
+        case 256 * 8 + 1: backward_rows<T, 256, 1, DROP>(a, s); break;
         case 256 * 8 + 2: backward_rows<T, 256, 2, DROP>(a, s); break;
-        case 256 * 8 + 4: backward_rows<T, 256, 4, DROP>(a, s); break;
-        case 512 * 8 + 4: backward_rows<T, 512, 4, DROP>(a, s); break;
-        default:
-            if (a.dx && a.rows) hipLaunchKernelGGL((k_norm_backward_rows<T, DROP>), dim3(grid_of(a.rows, 4, 256)), dim3(256), 0, s, a);
-            if (a.parts) hipLaunchKernelGGL((k_norm_backward_cols<T, DROP>), dim3((unsigned)((a.cols + 63) / 64) * (unsigned)a.parts), dim3(256), 0, s, a);
+        case 512 * 8 + 2: backward_rows<T, 512, 2, DROP>(a, s); break;
+        case NARROW: hipLaunchKernelGGL((k_norm_backward_narrow<T, DROP>), dim3(a.parts ? (unsigned)a.parts : grid_of(a.rows, 256, 256)), dim3(256), 0, s, a); break;
+        default: {
+            const unsigned parts = (unsigned)col_parts(sizeof(T) == 4 ? GNNX_F32 : GNNX_BF16, a.rows, a.cols), grid = (unsigned)a.chunks * parts;
+            if (a.dx && a.rows) hipLaunchKernelGGL((k_norm_chunk_sums<T, DROP>), dim3(grid_of(a.rows * a.chunks, 1, CHUNK_LANES)), dim3(CHUNK_LANES), 0, s, a);
+            if (a.parts) hipLaunchKernelGGL((k_norm_chunk_backward<T, DROP, true>), dim3(grid), dim3(CHUNK_LANES), 0, s, a);
+            else if (a.rows) hipLaunchKernelGGL((k_norm_chunk_backward<T, DROP, false>), dim3(grid), dim3(CHUNK_LANES), 0, s, a);
+        }
     }
     if (a.parts) hipLaunchKernelGGL((k_norm_join<T>), dim3((unsigned)((2 * a.cols + 31) / 32)), dim3(1024), 0, s, a);
 }
 
 }  // namespace
 
-extern "C" int gnnx_layer_norm_forward(const gnnx_norm* n, const gnnx_drop* drop, void* stream) {
+extern "C" size_t gnnx_layer_norm_workspace_bytes(int32_t type, int64_t rows, int64_t cols, int32_t backward) {
+    return type < 0 || type > 2 || rows < 0 || cols < 1 ? 0 : workspace_bytes_of(type, rows, cols, backward != 0);
+}
+
+extern "C" int gnnx_layer_norm_forward(const gnnx_norm* n, const gnnx_drop* drop, void* workspace, size_t workspace_bytes, void* stream) {
     NormArgs a;
     if (const char* e = norm_args(n, &a)) return set_error(e);
     if (const char* e = drop_args(drop, &a.drop)) return set_error(e);
@@ -168,16 +200,17 @@ extern "C" int gnnx_layer_norm_forward(const gnnx_norm* n, const gnnx_drop* drop
     if ((a.d != nullptr) != (drop != nullptr)) return set_error("layer norm: a dropped output and its dropout go together");
     if ((a.mean != nullptr) != (a.rstd != nullptr)) return set_error("layer norm: mean and rstd go together");
     if (!a.x) return set_error("null argument");
+    const RowShape sh = forward_shape(n->type, a.cols);
+    if (sh.lanes == LONG) {
+        if (!workspace || workspace_bytes < workspace_bytes_of(n->type, a.rows, a.cols, false)) return set_error("workspace too small");
+        a.chunk = static_cast<float*>(workspace);
+        a.chunks = chunks_of(n->type, a.cols);
+    }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (n->type == GNNX_F32) a.d ? run_forward<float, true>(a, s) : run_forward<float, false>(a, s);
-    else if (n->type == GNNX_BF16) a.d ? run_forward<bf16_t, true>(a, s) : run_forward<bf16_t, false>(a, s);
-    else a.d ? run_forward<f16_t, true>(a, s) : run_forward<f16_t, false>(a, s);
+    if (n->type == GNNX_F32) a.d ? run_forward<float, true>(a, sh, s) : run_forward<float, false>(a, sh, s);
+    else if (n->type == GNNX_BF16) a.d ? run_forward<bf16_t, true>(a, sh, s) : run_forward<bf16_t, false>(a, sh, s);
+    else a.d ? run_forward<f16_t, true>(a, sh, s) : run_forward<f16_t, false>(a, sh, s);
     return launched("gnnx_layer_norm_forward");
-}
-
-extern "C" size_t gnnx_layer_norm_workspace_bytes(int32_t type, int64_t rows, int64_t cols) {
-    if (rows < 0 || cols < 1) return 0;
-    return (size_t)col_parts(type, rows, cols) * 2 * (size_t)cols * sizeof(float);
 }
 
 extern "C" int gnnx_layer_norm_backward(const gnnx_norm* n, const gnnx_drop* drop, void* workspace, size_t workspace_bytes, void* stream) {
@@ -187,31 +220,55 @@ extern "C" int gnnx_layer_norm_backward(const gnnx_norm* n, const gnnx_drop* dro
     if (!a.dx && !a.dw && !a.db) return 0;
     if (a.rows > 0 && (a.dd != nullptr) != (drop != nullptr)) return set_error("layer norm: the gradient of a dropped output and its dropout go together");
     if (a.rows > 0 && ((!a.dy && !a.dd) || !a.x || !a.mean || !a.rstd)) return set_error("null argument");
+    const RowShape sh = backward_shape(n->type, a.cols);
+    const size_t needed = workspace_bytes_of(n->type, a.rows, a.cols, true);
+    if ((a.dw || a.db || sh.lanes == LONG) && (!workspace || workspace_bytes < needed)) return set_error("workspace too small");
     if (a.dw || a.db) {
-        if (!workspace || workspace_bytes < gnnx_layer_norm_workspace_bytes(n->type, a.rows, a.cols)) return set_error("workspace too small");
         a.part = static_cast<float*>(workspace);
         a.parts = col_parts(n->type, a.rows, a.cols);
     }
+    if (sh.lanes == LONG) {
+        a.chunk = reinterpret_cast<float*>(static_cast<char*>(workspace) + (needed - chunk_bytes(n->type, a.rows, a.cols)));
+        a.chunks = chunks_of(n->type, a.cols);
+    }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const RowShape sh = backward_shape(n->type, a.cols);
     if (n->type == GNNX_F32) a.dd ? run_backward<float, true>(a, sh, s) : run_backward<float, false>(a, sh, s);
     else if (n->type == GNNX_BF16) a.dd ? run_backward<bf16_t, true>(a, sh, s) : run_backward<bf16_t, false>(a, sh, s);
     else a.dd ? run_backward<f16_t, true>(a, sh, s) : run_backward<f16_t, false>(a, sh, s);
     return launched("gnnx_layer_norm_backward");
 }
 
+namespace {
+template <class T>
+void run_dropout(const DropoutArgs& a, hipStream_t s) {
+    const int64_t n = a.rows * (int64_t)a.pieces;
+    if (a.cols < Piece<T>::V) hipLaunchKernelGGL((k_dropout_narrow<T>), dim3(grid_of(a.rows, 256, 256)), dim3(256), 0, s, a);
+    else if (n >= (int64_t(1) << 32)) hipLaunchKernelGGL((k_dropout<T, true>), dim3(grid_of(n, 256, 256)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_dropout<T, false>), dim3(grid_of(n, 256, 256)), dim3(256), 0, s, a);
+}
+}  // namespace
+
 extern "C" int gnnx_dropout(int32_t type, int64_t rows, int64_t cols, const void* x, int64_t x_stride, void* y, const gnnx_drop* drop, void* stream) {
-    DropArgs d;
+    DropoutArgs a{};
     if (type < 0 || type > 2) return set_error("dropout: type must be 0 (fp32), 1 (bf16) or 2 (fp16)");
     if (!drop) return set_error("null argument");
-    if (const char* e = drop_args(drop, &d)) return set_error(e);
+    if (const char* e = drop_args(drop, &a.drop)) return set_error(e);
     if (rows < 0 || cols < 0 || x_stride < 0 || cols >= (int64_t(1) << 34)) return set_error("dropout: needs rows, stride >= 0 and 0 <= cols < 2^34");
     if (rows == 0 || cols == 0) return 0;
     if (!x || !y) return set_error("null argument");
+    a.rows = rows;
+    a.cols = cols;
+    a.stride = x_stride;
+    a.x = x;
+    a.y = y;
+    const uint64_t d = (uint64_t)pieces_of(type, cols);      // < 2^32
+    a.pieces = (uint32_t)d;
+    // division by d of any n < 2^32: with 2^shift the power of two at or above d, magic = floor(2^32 (2^shift - d) / d) + 1
+    while ((uint64_t(1) << a.shift) < d) ++a.shift;
+    a.magic = (uint32_t)((((uint64_t(1) << a.shift) - d) << 32) / d + 1);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const dim3 grid(grid_of(rows * ((cols + 3) / 4), 256, 256)), block(256);
-    if (type == GNNX_F32) hipLaunchKernelGGL((k_dropout<float>), grid, block, 0, s, rows, cols, x_stride, static_cast<const float*>(x), static_cast<float*>(y), d);
-    else if (type == GNNX_BF16) hipLaunchKernelGGL((k_dropout<bf16_t>), grid, block, 0, s, rows, cols, x_stride, static_cast<const bf16_t*>(x), static_cast<bf16_t*>(y), d);
-    else hipLaunchKernelGGL((k_dropout<f16_t>), grid, block, 0, s, rows, cols, x_stride, static_cast<const f16_t*>(x), static_cast<f16_t*>(y), d);
+    if (type == GNNX_F32) run_dropout<float>(a, s);
+    else if (type == GNNX_BF16) run_dropout<bf16_t>(a, s);
+    else run_dropout<f16_t>(a, s);
     return launched("gnnx_dropout");
 }

@@ -207,8 +207,8 @@ _API = {
     "gnnx_set_mt_jump_poly": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64]),
     "gnnx_set_mt_jump_polys": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32]),
     "gnnx_xl_run": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(_Hyper), ctypes.POINTER(_XlState)] + [ctypes.c_void_p] * 5),
-    "gnnx_layer_norm_forward": (ctypes.c_int, [ctypes.POINTER(_Norm), ctypes.POINTER(_Drop), ctypes.c_void_p]),
-    "gnnx_layer_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int64, ctypes.c_int64]),
+    "gnnx_layer_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]),
+    "gnnx_layer_norm_forward": (ctypes.c_int, [ctypes.POINTER(_Norm), ctypes.POINTER(_Drop), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "gnnx_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(_Norm), ctypes.POINTER(_Drop), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "gnnx_dropout": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.POINTER(_Drop),
                                     ctypes.c_void_p]),

@@ -129,6 +129,14 @@ def _param(p):
     return p if p is None or p.is_contiguous() else p.contiguous()
 
 
+_SHORT = 4096      # rows of no more columns never need scratch of their own
+
+
+def _workspace(lib, x, rows, cols, backward):
+    nb = lib.gnnx_layer_norm_workspace_bytes(_TYPES[x.dtype], rows, cols, backward)
+    return torch.empty(nb, dtype=torch.uint8, device=x.device), nb
+
+
 def _norm_forward(x, weight, bias, eps, relu, drop, stats):
     """-> (y, d or None, mean or None, rstd or None); drop: None or the tuple (p, seed, step, row_offset)"""
     _check_norm(x, weight, bias)
@@ -148,7 +156,8 @@ def _norm_forward(x, weight, bias, eps, relu, drop, stats):
     par = weight if weight is not None else bias
     a = _Norm(_TYPES[x.dtype], int(par is not None and par.dtype == torch.float32), rows, cols, stride, 0, 0, xm.data_ptr(), _ptr(weight), _ptr(bias), None, None,
               y.data_ptr(), _ptr(out), None, None, None, _ptr(mean), _ptr(rstd), eps, int(bool(relu)))
-    _call(x, lib.gnnx_layer_norm_forward, lib, a, d)
+    ws, nb = _workspace(lib, x, rows, cols, 0) if cols > _SHORT else (None, 0)
+    _call(x, lib.gnnx_layer_norm_forward, lib, a, d, _ptr(ws), nb)
     return y, out, mean, rstd
 
 
@@ -169,10 +178,7 @@ def _norm_backward(dy, dd, x, mean, rstd, weight, relu, drop, need, param_dtype)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
     dw = torch.empty(cols, dtype=param_dtype, device=x.device) if need[1] else None
     db = torch.empty(cols, dtype=param_dtype, device=x.device) if need[2] else None
-    ws, nb = None, 0
-    if need[1] or need[2]:
-        nb = lib.gnnx_layer_norm_workspace_bytes(_TYPES[x.dtype], rows, cols)
-        ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+    ws, nb = _workspace(lib, x, rows, cols, 1) if need[1] or need[2] or cols > _SHORT else (None, 0)
     a = _Norm(_TYPES[x.dtype], int(param_dtype == torch.float32), rows, cols, stride, dys, dds, xm.data_ptr(), _ptr(weight), None, _ptr(dym), _ptr(ddm),
               None, None, _ptr(dx), _ptr(dw), _ptr(db), mean.data_ptr(), rstd.data_ptr(), 0.0, int(bool(relu)))
     _call(x, lib.gnnx_layer_norm_backward, lib, a, d, _ptr(ws), nb)

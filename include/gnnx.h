@@ -454,10 +454,11 @@ typedef struct {
     float eps;                              /* >= 0 (forward) */
     int32_t relu;                           /* backward: dx = 0 where x <= 0 */
 } gnnx_norm;
-int gnnx_layer_norm_forward(const gnnx_norm* n, const gnnx_drop* drop, void* stream);
-/* workspace: DEVICE scratch of gnnx_layer_norm_workspace_bytes(type, rows, cols) bytes, or NULL where neither dw nor db is asked for.  dw and db are summed in
- * an order that the sizes alone decide: the same inputs give the same bits. */
-size_t gnnx_layer_norm_workspace_bytes(int32_t type, int64_t rows, int64_t cols);
+/* workspace: DEVICE scratch of gnnx_layer_norm_workspace_bytes(type, rows, cols, backward) bytes, the call's own until it has run (forward: 0 bytes = NULL for all but
+ * rows too long for a workgroup; backward: NULL also where neither dw nor db is asked for and the rows are not too long).  dw and db are summed in an order that the sizes
+ * alone decide: the same inputs give the same bits. */
+size_t gnnx_layer_norm_workspace_bytes(int32_t type, int64_t rows, int64_t cols, int32_t backward);
+int gnnx_layer_norm_forward(const gnnx_norm* n, const gnnx_drop* drop, void* workspace, size_t workspace_bytes, void* stream);
 int gnnx_layer_norm_backward(const gnnx_norm* n, const gnnx_drop* drop, void* workspace, size_t workspace_bytes, void* stream);
 /* y = dropout(x), y contiguous; its backward pass is the same call on the gradient. */
 int gnnx_dropout(int32_t type, int64_t rows, int64_t cols, const void* x, int64_t x_stride, void* y, const gnnx_drop* drop, void* stream);

@@ -72,6 +72,9 @@ inline void __threadfence_block() {}
 // DPP row_shl:S (dpp_ctrl 0x100 + S, all rows / banks, bound_ctrl): lane l <- lane l + S of its 16-lane row, else 0
 inline int emu_update_dpp(int old, int src, int ctrl, int row_mask, int bank_mask, bool bound_ctrl) {
     (void)old; (void)row_mask; (void)bank_mask; (void)bound_ctrl;
+    if (ctrl < 0x100) return emu::shfl_i(src, (int)(threadIdx.x & 60u) + ((ctrl >> (2 * (threadIdx.x & 3u))) & 3));   // quad_perm
+    if (ctrl == 0x140) return emu::shfl_xor_i(src, 15);                                       // row_mirror: lane l <- 15 - l of its row
+    if (ctrl == 0x141) return emu::shfl_xor_i(src, 7);                                        // row_half_mirror: 7 - l of its half row
     if (ctrl > 0x120 && ctrl < 0x130) return emu::dpp_row_ror(src, ctrl - 0x120);   // row_ror:S
     return emu::dpp_row_shl(src, ctrl - 0x100);
 }

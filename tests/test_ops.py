@@ -421,13 +421,14 @@ def test_the_c_entry_points_refuse_what_they_cannot_do(be):
             setattr(n, k, v)
         return n
     drop = engine._Drop(0.5, 1, None, 0, 0)
+    assert lib.gnnx_layer_norm_forward(norm(rows=1, cols=1 << 20, x_stride=1 << 20), None, None, 0, None) != 0      # a long row without its workspace
     bad = [norm(type=3), norm(type=-1), norm(rows=-1), norm(cols=0), norm(cols=1 << 30), norm(x_stride=-8), norm(eps=-1.0), norm(y=None), norm(x=None),
            norm(mean=out.data_ptr()), norm(d=out.data_ptr())]
     for n in bad:
-        assert lib.gnnx_layer_norm_forward(n, None, None) != 0 and len(lib.gnnx_last_error()) > 5
-    assert lib.gnnx_layer_norm_forward(None, None, None) != 0
-    assert lib.gnnx_layer_norm_forward(norm(), drop, None) != 0
-    assert lib.gnnx_layer_norm_forward(norm(d=out.data_ptr()), engine._Drop(1.5, 1, None, 0, 0), None) != 0
+        assert lib.gnnx_layer_norm_forward(n, None, None, 0, None) != 0 and len(lib.gnnx_last_error()) > 5
+    assert lib.gnnx_layer_norm_forward(None, None, None, 0, None) != 0
+    assert lib.gnnx_layer_norm_forward(norm(), drop, None, 0, None) != 0
+    assert lib.gnnx_layer_norm_forward(norm(d=out.data_ptr()), engine._Drop(1.5, 1, None, 0, 0), None, 0, None) != 0
     for n, ws in ((norm(dw=out.data_ptr(), dy=x.data_ptr(), mean=out.data_ptr(), rstd=out.data_ptr()), 0), (norm(dx=out.data_ptr()), 0),
                   (norm(dx=out.data_ptr(), dy=x.data_ptr()), 0), (norm(dx=out.data_ptr(), dd=x.data_ptr(), mean=out.data_ptr(), rstd=out.data_ptr()), 0)):
         assert lib.gnnx_layer_norm_backward(n, None, None, ws, None) != 0
