@@ -11,6 +11,10 @@
 #pragma once
 #include <stdint.h>
 
+// No contraction by the compiler: every fma below is written out, so the variants of a kernel (with or without dropout, with or without the parameters' gradients,
+// whatever the shape of the launch adds up first) round an element alike.
+#pragma clang fp contract(off)
+
 namespace gnnx {
 
 typedef __bf16 bf16_t;
@@ -84,7 +88,9 @@ __device__ __forceinline__ float param_at(const void* p, int32_t is_f32, int64_t
 // A row is shared by TPR lanes (beyond 64: threads of a workgroup); each holds K pieces of 16 bytes, V elements.  Piece k of lane l is meant to start at column
 // (k TPR + l) V; one that would reach past the row starts at cols - V instead and leaves out of every sum the `skip` elements that the piece before it has as
 // well (a piece wholly beyond the row leaves out all V).  So every access is one 16-byte access inside the row, whatever the row's length and alignment (the
-// hardware takes any alignment): no tail, no variant for odd rows or slices.  Both holders of an element store the same value.  Needs cols >= V.
+// hardware takes any alignment): no tail, no variant for odd rows or slices, no branch around a store - both holders of an element compute and store the same
+// bits, and so do lanes whose row lies beyond the last, which repeat that one.  Needs cols >= V.  K is the least that holds the row: only the last round of
+// pieces can reach past it.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <class T>
 struct Piece {
@@ -96,14 +102,15 @@ struct Piece {
         else return (float)__builtin_bit_cast(f16_t, (uint16_t)(j & 1 ? w[j >> 1] >> 16 : w[j >> 1]));
     }
 };
+// (column c of a row: a 32-bit byte offset from the row's start, which is the same for a whole wave in all but the narrow shapes - one scalar base per row)
 template <class T>
-__device__ __forceinline__ Piece<T> load_piece(const T* p) {
+__device__ __forceinline__ Piece<T> load_piece(const void* row, uint32_t c) {
     Piece<T> q;
-    __builtin_memcpy(&q.w, p, 16);
+    __builtin_memcpy(&q.w, static_cast<const char*>(row) + c * (uint32_t)sizeof(T), 16);
     return q;
 }
 template <class T>
-__device__ __forceinline__ void store_piece(T* p, const float* v) {
+__device__ __forceinline__ void store_piece(void* row, uint32_t c, const float* v) {
     Piece<T> q;
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -113,41 +120,39 @@ __device__ __forceinline__ void store_piece(T* p, const float* v) {
         for (int j = 0; j < 4; ++j)
             q.w[j] = (uint32_t)__builtin_bit_cast(uint16_t, (T)v[2 * j]) | (uint32_t)__builtin_bit_cast(uint16_t, (T)v[2 * j + 1]) << 16;
     }
-    __builtin_memcpy(p, &q.w, 16);
+    __builtin_memcpy(static_cast<char*>(row) + c * (uint32_t)sizeof(T), &q.w, 16);
 }
-// the V parameters of a piece (fp32, or x's type)
-template <class T>
-__device__ __forceinline__ void load_params(float* out, const void* p, int32_t is_f32, int64_t c) {
-    constexpr int V = Piece<T>::V;
-    if (sizeof(T) == 4 || is_f32) {
+// the V parameters (of type P: fp32, or x's type) of a piece of x
+template <class T, class P>
+struct Params {
+    static constexpr int N = (int)(sizeof(P) / sizeof(T));
+    Piece<P> q[N];
+    __device__ __forceinline__ void load(const void* p, uint32_t c) {
 #pragma unroll
-        for (int h = 0; h < V; h += 4) {
-            const Piece<float> q = load_piece(static_cast<const float*>(p) + c + h);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) out[h + j] = q.at(j);
-        }
-    } else {
-        const Piece<T> q = load_piece(static_cast<const T*>(p) + c);
-#pragma unroll
-        for (int j = 0; j < V; ++j) out[j] = q.at(j);
+        for (int i = 0; i < N; ++i) q[i] = load_piece<P>(p, c + i * Piece<P>::V);
     }
-}
-struct Slot { int64_t c; int skip; };
+    __device__ __forceinline__ void ones() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) q[i].w = (u32x4)(sizeof(P) == 4 ? 0x3f800000u : __is_same(P, bf16_t) ? 0x3f803f80u : 0x3c003c00u);
+    }
+    __device__ __forceinline__ float at(int j) const { return q[j / Piece<P>::V].at(j % Piece<P>::V); }
+};
+struct Slot { uint32_t c; int skip; };
 template <int V>
-__device__ __forceinline__ Slot slot_at(int64_t c, int64_t cols) {
-    const int64_t last = cols - V, over = c - last;
-    return over <= 0 ? Slot{c, 0} : Slot{last, over < V ? (int)over : V};
+__device__ __forceinline__ Slot slot_at(uint32_t c, uint32_t cols) {      // cols < 2^30
+    const int over = (int)c - (int)(cols - V);
+    return over <= 0 ? Slot{c, 0} : Slot{cols - V, over < V ? over : V};
 }
 
 // The dropout of a piece's V elements from column c on (c is a multiple of 4 unless the piece was moved back from the end of a row that 4 does not divide:
 // its words then lie across V / 4 + 1 blocks).
 template <class T>
-__device__ __forceinline__ void drop_piece(const DropArgs& d, const DropKey& key, int64_t r, int64_t c, int64_t cols, float* v) {
+__device__ __forceinline__ void drop_piece(const DropArgs& d, const DropKey& key, int64_t r, uint32_t c, uint32_t cols, float* v) {
     constexpr int V = Piece<T>::V;
     if ((cols & 3) == 0) {
 #pragma unroll
         for (int h = 0; h < V; h += 4) {
-            const Philox4 q = drop_words(d, key, r, (uint32_t)(c >> 2) + h / 4);
+            const Philox4 q = drop_words(d, key, r, (c >> 2) + h / 4);
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[h + j] = dropped(d, q.w[j], v[h + j]);
         }
@@ -155,7 +160,7 @@ __device__ __forceinline__ void drop_piece(const DropArgs& d, const DropKey& key
         uint32_t w[V + 4];
 #pragma unroll
         for (int h = 0; h < V + 4; h += 4) {
-            const Philox4 q = drop_words(d, key, r, (uint32_t)(c >> 2) + h / 4);
+            const Philox4 q = drop_words(d, key, r, (c >> 2) + h / 4);
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[h + j] = q.w[j];
         }
@@ -220,25 +225,39 @@ __device__ __forceinline__ void row_totals(float (&v)[N], float (*part)[N]) {
 }
 
 // y (and d) of one piece from its xhat
-template <class T, bool DROP>
-__device__ __forceinline__ void norm_outputs(const NormArgs& a, const DropKey& key, int64_t r, int64_t c, float* v) {
+template <class T, class P, bool DROP>
+__device__ __forceinline__ void norm_outputs(const NormArgs& a, const DropKey& key, int64_t r, uint32_t c, const Params<T, P>& w, const Params<T, P>& b, float* v) {
     constexpr int V = Piece<T>::V;
-    float p[V];
-    if (a.w) {
-        load_params<T>(p, a.w, a.w_is_f32, c);
+    if (a.w && a.b) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] *= p[j];
-    }
-    if (a.b) {
-        load_params<T>(p, a.b, a.w_is_f32, c);
+        for (int j = 0; j < V; ++j) v[j] = __builtin_fmaf(v[j], w.at(j), b.at(j));
+    } else if (a.w) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] += p[j];
+        for (int j = 0; j < V; ++j) v[j] *= w.at(j);
+    } else if (a.b) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] += b.at(j);
     }
-    if (a.y) store_piece(static_cast<T*>(a.y) + r * a.cols + c, v);
+    if (a.y) store_piece<T>(static_cast<T*>(a.y) + r * a.cols, c, v);
     if (DROP) {
-        drop_piece<T>(a.drop, key, r, c, a.cols, v);
-        store_piece(static_cast<T*>(a.d) + r * a.cols + c, v);
+        drop_piece<T>(a.drop, key, r, c, (uint32_t)a.cols, v);
+        store_piece<T>(static_cast<T*>(a.d) + r * a.cols, c, v);
     }
+}
+
+// the row of a lane among those its workgroup works on at once
+template <int TPR>
+__device__ __forceinline__ int row_in_group() {
+    if constexpr (TPR > 64) return 0;
+    else if constexpr (TPR == 64) return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    else return (int)(threadIdx.x / TPR);
+}
+
+// ... and the row itself: the last one for lanes beyond it
+template <int TPR>
+__device__ __forceinline__ int64_t row_of(int64_t r0, int64_t rows) {
+    const int64_t r = r0 + row_in_group<TPR>();
+    return r < rows ? r : rows - 1;
 }
 
 template <int TPR>
@@ -251,7 +270,7 @@ __device__ __forceinline__ float pieces_sum(const Piece<T> (&q)[K], const Slot (
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         Piece<T> p = q[k];
-        if (2 * k + 1 >= K) p.w &= piece_mask<T>(at[k].skip);      // (more than half of the K rounds are full: the launch's choice of K)
+        if (k + 1 == K) p.w &= piece_mask<T>(at[k].skip);
 #pragma unroll
         for (int j = 0; j < Piece<T>::V; ++j) s += floored(p.at(j), floor);
     }
@@ -265,12 +284,12 @@ __device__ __forceinline__ float pieces_squares(const Piece<T> (&q)[K], const Sl
 #pragma unroll
         for (int j = 0; j < Piece<T>::V; ++j) {
             const float v = floored(q[k].at(j), floor) - mean;
-            s += 2 * k + 1 < K || j >= at[k].skip ? v * v : 0.0f;
+            s = k + 1 < K || j >= at[k].skip ? __builtin_fmaf(v, v, s) : s;
         }
     return s;
 }
 
-template <class T, int TPR, int K, bool DROP>
+template <class T, class P, int TPR, int K, bool DROP>
 __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a) {
     constexpr int V = Piece<T>::V, RPB = norm_threads<TPR>() / TPR;
     __shared__ float part[2][TPR > 64 ? TPR / 64 : 1][1];
@@ -278,35 +297,39 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
     const float inv = 1.0f / (float)a.cols;
     const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
-        const bool live = r0 + threadIdx.x / TPR < a.rows;      // (a workgroup of one row is live as a whole)
-        const int64_t r = live ? r0 + threadIdx.x / TPR : a.rows - 1;
+        const int64_t r = row_of<TPR>(r0, a.rows);
         const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
         Piece<T> q[K];                             // as stored: widened again in each pass, half the registers for 16-bit types
+        Params<T, P> w[K], b[K];                   // on their way with the row: nothing of the chain load - mean - variance - store waits for them
         Slot at[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            at[k] = slot_at<V>((k * TPR + l) * V, a.cols);
-            q[k] = load_piece(x + at[k].c);
+            at[k] = slot_at<V>((k * TPR + l) * V, (uint32_t)a.cols);
+            q[k] = load_piece<T>(x, at[k].c);
         }
+        if (a.w)
+#pragma unroll
+            for (int k = 0; k < K; ++k) w[k].load(a.w, at[k].c);
+        if (a.b)
+#pragma unroll
+            for (int k = 0; k < K; ++k) b[k].load(a.b, at[k].c);
         float s[1] = {pieces_sum(q, at, a.relu_floor)};
         row_totals<TPR>(s, part[0]);
         const float mean = s[0] * inv;
         s[0] = pieces_squares(q, at, a.relu_floor, mean);
         row_totals<TPR>(s, part[1]);
         const float rstd = 1.0f / sqrtf(s[0] * inv + a.eps);
-        if (!live) continue;
         if (l == 0 && a.mean) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
         }
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (at[k].skip < V) {
-                float v[V];
+        for (int k = 0; k < K; ++k) {
+            float v[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[j] = (floored(q[k].at(j), a.relu_floor) - mean) * rstd;
-                norm_outputs<T, DROP>(a, key, r, at[k].c, v);
-            }
+            for (int j = 0; j < V; ++j) v[j] = (floored(q[k].at(j), a.relu_floor) - mean) * rstd;
+            norm_outputs<T, P, DROP>(a, key, r, at[k].c, w[k], b[k], v);
+        }
     }
 }
 
@@ -319,7 +342,7 @@ template <class T>
 __device__ __forceinline__ void chunk_slots(Slot (&at)[CHUNK_PIECES], int ch, int64_t cols) {
 #pragma unroll
     for (int k = 0; k < CHUNK_PIECES; ++k)
-        at[k] = slot_at<Piece<T>::V>((int64_t)ch * chunk_cols<T>() + (k * CHUNK_LANES + (int)threadIdx.x) * Piece<T>::V, cols);
+        at[k] = slot_at<Piece<T>::V>((uint32_t)ch * chunk_cols<T>() + (k * CHUNK_LANES + threadIdx.x) * Piece<T>::V, (uint32_t)cols);
 }
 
 // First launch of the forward pass: the chunk's mean and its sum of squared distances from that mean.
@@ -334,7 +357,7 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_stats(NormArgs a) {
         Piece<T> q[CHUNK_PIECES];
         chunk_slots<T>(at, ch, a.cols);
 #pragma unroll
-        for (int k = 0; k < CHUNK_PIECES; ++k) q[k] = load_piece(static_cast<const T*>(a.x) + r * a.x_stride + at[k].c);
+        for (int k = 0; k < CHUNK_PIECES; ++k) q[k] = load_piece<T>(static_cast<const T*>(a.x) + r * a.x_stride, at[k].c);
         float s[1] = {0.0f};
 #pragma unroll
         for (int k = 0; k < CHUNK_PIECES; ++k) {
@@ -352,7 +375,7 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_stats(NormArgs a) {
 #pragma unroll
             for (int j = 0; j < Piece<T>::V; ++j) {
                 const float v = floored(q[k].at(j), a.relu_floor) - mean;
-                s[0] += j >= at[k].skip ? v * v : 0.0f;
+                s[0] = j >= at[k].skip ? __builtin_fmaf(v, v, s[0]) : s[0];
             }
         row_totals<CHUNK_LANES>(s, part[1]);
         if (threadIdx.x == 0) {
@@ -364,7 +387,7 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_stats(NormArgs a) {
 
 // Second launch: the row's statistics from its chunks' - sum of squares = sum of the chunks' + their sizes times the squared distance of their means from the
 // row's - in every workgroup alike, then the chunk's outputs.
-template <class T, bool DROP>
+template <class T, class P, bool DROP>
 __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_outputs(NormArgs a) {
     const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
     const int64_t units = a.rows * a.chunks;
@@ -375,7 +398,7 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_outputs(NormArgs a) 
         Piece<T> q[CHUNK_PIECES];
         chunk_slots<T>(at, ch, a.cols);
 #pragma unroll
-        for (int k = 0; k < CHUNK_PIECES; ++k) q[k] = load_piece(static_cast<const T*>(a.x) + r * a.x_stride + at[k].c);
+        for (int k = 0; k < CHUNK_PIECES; ++k) q[k] = load_piece<T>(static_cast<const T*>(a.x) + r * a.x_stride, at[k].c);
         const float* st = a.chunk + 2 * r * a.chunks;
         const int lane = threadIdx.x & 63;
         float s = 0.0f;
@@ -396,13 +419,15 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_outputs(NormArgs a) 
             a.rstd[r] = rstd;
         }
 #pragma unroll
-        for (int k = 0; k < CHUNK_PIECES; ++k)
-            if (at[k].skip < Piece<T>::V) {
-                float v[Piece<T>::V];
+        for (int k = 0; k < CHUNK_PIECES; ++k) {
+            float v[Piece<T>::V];
 #pragma unroll
-                for (int j = 0; j < Piece<T>::V; ++j) v[j] = (floored(q[k].at(j), a.relu_floor) - mean) * rstd;
-                norm_outputs<T, DROP>(a, key, r, at[k].c, v);
-            }
+            for (int j = 0; j < Piece<T>::V; ++j) v[j] = (floored(q[k].at(j), a.relu_floor) - mean) * rstd;
+            Params<T, P> w, b;
+            if (a.w) w.load(a.w, at[k].c);
+            if (a.b) b.load(a.b, at[k].c);
+            norm_outputs<T, P, DROP>(a, key, r, at[k].c, w, b, v);
+        }
     }
 }
 
@@ -419,7 +444,7 @@ __global__ __launch_bounds__(256) void k_norm_forward_narrow(NormArgs a) {
         s = 0.0f;
         for (int c = 0; c < a.cols; ++c) {
             const float v = floored((float)x[c], a.relu_floor) - mean;
-            s += v * v;
+            s = __builtin_fmaf(v, v, s);
         }
         const float rstd = 1.0f / sqrtf(s * inv + a.eps);
         if (a.mean) {
@@ -428,8 +453,8 @@ __global__ __launch_bounds__(256) void k_norm_forward_narrow(NormArgs a) {
         }
         for (int c = 0; c < a.cols; ++c) {
             float v = (floored((float)x[c], a.relu_floor) - mean) * rstd;
-            if (a.w) v *= param_at<T>(a.w, a.w_is_f32, c);
-            if (a.b) v += param_at<T>(a.b, a.w_is_f32, c);
+            const float w = a.w ? param_at<T>(a.w, a.w_is_f32, c) : 1.0f;
+            v = a.b ? __builtin_fmaf(v, w, param_at<T>(a.b, a.w_is_f32, c)) : v * w;
             if (a.y) static_cast<T*>(a.y)[r * a.cols + c] = (T)v;
             if (DROP) static_cast<T*>(a.d)[r * a.cols + c] = (T)dropped(a.drop, drop_words(a.drop, key, r, (uint32_t)(c >> 2)).w[c & 3], v);
         }
@@ -437,70 +462,66 @@ __global__ __launch_bounds__(256) void k_norm_forward_narrow(NormArgs a) {
 }
 
 // ---- backward ----
-// What a lane holds of one row: its pieces of x, dy and dd as stored.  Where a piece was moved back, dy and dd are blanked in the elements that count elsewhere:
-// they then add nothing to any sum, and only the elements that count are stored.
+// What a lane holds of one row: its pieces of x, dy and dd as stored.
 template <class T, int K, bool DROP>
 struct RowPieces {
+    static constexpr int V = Piece<T>::V;
     Piece<T> x[K], dy[K], dd[DROP ? K : 1];
     float mean, rstd;
-    __device__ __forceinline__ void load(const NormArgs& a, const Slot (&at)[K], int64_t r, bool live) {
-        const T* xr = static_cast<const T*>(a.x) + r * a.x_stride;
+    __device__ __forceinline__ void load(const NormArgs& a, const Slot (&at)[K], int64_t r) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) x[k] = load_piece(xr + at[k].c);
+        for (int k = 0; k < K; ++k) x[k] = load_piece<T>(static_cast<const T*>(a.x) + r * a.x_stride, at[k].c);
+        if constexpr (DROP) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            if (a.dy) dy[k] = load_piece(static_cast<const T*>(a.dy) + r * a.dy_stride + at[k].c);
-            else dy[k].w = (u32x4)0u;
-            if constexpr (DROP) dd[k] = load_piece(static_cast<const T*>(a.dd) + r * a.dd_stride + at[k].c);
+            for (int k = 0; k < K; ++k) dd[k] = load_piece<T>(static_cast<const T*>(a.dd) + r * a.dd_stride, at[k].c);
+        }
+        if (!DROP || a.dy) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) dy[k] = load_piece<T>(static_cast<const T*>(a.dy) + r * a.dy_stride, at[k].c);
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k) dy[k].w = (u32x4)0u;
         }
         mean = a.mean[r];
         rstd = a.rstd[r];
-        if (!live) {
+    }
+    // the dropped output's share of dL/dy, formed once per row
+    __device__ __forceinline__ void dropped_share(const NormArgs& a, const DropKey& key, const Slot (&at)[K], int64_t r, float (&d)[DROP ? K : 1][V]) const {
+        if constexpr (DROP) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                dy[k].w = (u32x4)0u;
-                if constexpr (DROP) dd[k].w = (u32x4)0u;
+#pragma unroll
+                for (int j = 0; j < V; ++j) d[k][j] = dd[k].at(j);
+                drop_piece<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, d[k]);
             }
         }
     }
-    // dL/dy of piece k
-    __device__ __forceinline__ void gradient(const NormArgs& a, const DropKey& key, const Slot& at, const u32x4& mask, int64_t r, int k, float* g) {
+    __device__ __forceinline__ float xhat(const NormArgs& a, int k, int j) const { return (floored(x[k].at(j), a.relu_floor) - mean) * rstd; }
+    // dL/dy of piece k: MASKED, 0 in the elements that do not count here
+    template <bool MASKED>
+    __device__ __forceinline__ void gradient(int k, const u32x4& mask, int skip, const float (&d)[DROP ? K : 1][V], float* g) const {
         Piece<T> p = dy[k];
-        if (2 * k + 1 >= K) p.w &= mask;
+        if (MASKED) p.w &= mask;
 #pragma unroll
-        for (int j = 0; j < Piece<T>::V; ++j) g[j] = p.at(j);
-        if constexpr (DROP) {
-            Piece<T> e = dd[k];
-            if (2 * k + 1 >= K) e.w &= mask;
-            float d[Piece<T>::V];
-#pragma unroll
-            for (int j = 0; j < Piece<T>::V; ++j) d[j] = e.at(j);
-            drop_piece<T>(a.drop, key, r, at.c, a.cols, d);
-#pragma unroll
-            for (int j = 0; j < Piece<T>::V; ++j) g[j] += d[j];
+        for (int j = 0; j < V; ++j) {
+            g[j] = p.at(j);
+            if constexpr (DROP) g[j] += !MASKED || j >= skip ? d[k][j] : 0.0f;
         }
     }
+    // dx of piece k from the row's c1, c2
+    template <class P>
+    __device__ __forceinline__ void store_dx(const NormArgs& a, int k, const Slot& at, int64_t r, const Params<T, P>& w, float c1, float c2,
+                                             const float (&d)[DROP ? K : 1][V]) const {
+        float g[V];
+        gradient<false>(k, (u32x4)0u, 0, d, g);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float v = rstd * __builtin_fmaf(-xhat(a, k, j), c2, g[j] * w.at(j) - c1);
+            g[j] = x[k].at(j) <= a.relu_stop ? 0.0f : v;
+        }
+        store_piece<T>(static_cast<T*>(a.dx) + r * a.cols, at.c, g);
+    }
 };
-
-// dx of one piece from g = dy w; a piece that was moved back stores its own elements only
-template <class T>
-__device__ __forceinline__ void store_dx(const NormArgs& a, const Piece<T>& x, const Slot& at, int64_t r, float mean, float rstd, float c1, float c2, const float* g) {
-    constexpr int V = Piece<T>::V;
-    float v[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const float xv = x.at(j), xhat = (floored(xv, a.relu_floor) - mean) * rstd, d = rstd * (g[j] - c1 - xhat * c2);
-        v[j] = xv <= a.relu_stop ? 0.0f : d;
-    }
-    T* out = static_cast<T*>(a.dx) + r * a.cols + at.c;
-    if (at.skip == 0) {
-        store_piece(out, v);
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j >= at.skip) out[j] = (T)v[j];
-    }
-}
 
 // a lane's partial sums of dw and db, of the columns that count with it
 template <int V>
@@ -516,7 +537,9 @@ __device__ __forceinline__ void store_cols(const NormArgs& a, int64_t part, cons
 
 // The backward pass of rows in registers: one pass over x, dy (and dd), dx out.  COLS: a workgroup walks rows a grid apart and keeps its share of dw and db in
 // registers; at the end the lanes that hold the same column add up (lane sums, then LDS across the waves) and the workgroup leaves one partial row of each.
-template <class T, int TPR, int K, bool DROP, bool COLS>
+// The next row is always on its way while one is worked on (the last one is loaded again at the end: a load that may or may not have been issued would make
+// the wait for the row before it a wait for everything).
+template <class T, class P, int TPR, int K, bool DROP, bool COLS>
 __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs a) {
     constexpr int V = Piece<T>::V, RPB = norm_threads<TPR>() / TPR;
     __shared__ float part[2][TPR > 64 ? TPR / 64 : 1][2];
@@ -524,64 +547,58 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs 
     const float inv = 1.0f / (float)a.cols;
     const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
     Slot at[K];
-    u32x4 mask[K];
+    Params<T, P> w[K];
     float sw[K][V], sb[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        at[k] = slot_at<V>((k * TPR + l) * V, a.cols);
-        mask[k] = piece_mask<T>(at[k].skip);
+        at[k] = slot_at<V>((k * TPR + l) * V, (uint32_t)a.cols);
+        if (a.w) w[k].load(a.w, at[k].c);
+        else w[k].ones();
 #pragma unroll
         for (int j = 0; j < V; ++j) sw[k][j] = sb[k][j] = 0.0f;
     }
-    int turn = 0;
+    const u32x4 mask = piece_mask<T>(at[K - 1].skip);
     const int64_t step = (int64_t)gridDim.x * RPB;
-    int64_t r0 = (int64_t)blockIdx.x * RPB;
-    const auto row_of = [&](int64_t base, bool* live) {
-        const int64_t r = base + threadIdx.x / TPR;
-        *live = RPB == 1 || r < a.rows;
-        return *live ? r : a.rows - 1;
-    };
-    RowPieces<T, K, DROP> now, next;
-    bool live, next_live;
-    int64_t r, next_r;
-    if (r0 < a.rows) {
-        r = row_of(r0, &live);
-        now.load(a, at, r, live);
-    }
-    for (; r0 < a.rows; r0 += step, turn ^= 1) {
-        if (r0 + step < a.rows) {                  // the next row is on its way while this one is worked on
-            next_r = row_of(r0 + step, &next_live);
-            next.load(a, at, next_r, next_live);
-        }
-        float g[K][V], s[2] = {0.0f, 0.0f};
+    const auto work = [&](const RowPieces<T, K, DROP>& now, int64_t r0, int turn) {
+        const int64_t r = row_of<TPR>(r0, a.rows);
+        const bool live = r0 + row_in_group<TPR>() < a.rows;
+        float d[DROP ? K : 1][V], s[2] = {0.0f, 0.0f};
+        now.dropped_share(a, key, at, r, d);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            now.gradient(a, key, at[k], mask[k], r, k, g[k]);
-            float p[V];
-            if (a.w) load_params<T>(p, a.w, a.w_is_f32, at[k].c);
+            float g[V], xhat[V];
+            if (k + 1 < K) now.template gradient<false>(k, mask, 0, d, g);
+            else now.template gradient<true>(k, mask, at[k].skip, d, g);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float xhat = (floored(now.x[k].at(j), a.relu_floor) - now.mean) * now.rstd;
-                if (COLS) {
-                    sb[k][j] += g[k][j];
-                    sw[k][j] += g[k][j] * xhat;
-                }
-                if (a.w) g[k][j] *= p[j];
-                s[0] += g[k][j];
-                s[1] += g[k][j] * xhat;
+                xhat[j] = now.xhat(a, k, j);
+                const float gw = g[j] * w[k].at(j);
+                s[0] += gw;
+                s[1] = __builtin_fmaf(gw, xhat[j], s[1]);
             }
-        }
-        if (a.dx) {
-            row_totals<TPR>(s, part[turn]);
-            const float c1 = s[0] * inv, c2 = s[1] * inv;
-            if (live)
+            if (COLS && (RPB == 1 || live))
 #pragma unroll
-                for (int k = 0; k < K; ++k)
-                    if (at[k].skip < V) store_dx(a, now.x[k], at[k], r, now.mean, now.rstd, c1, c2, g[k]);
+                for (int j = 0; j < V; ++j) {
+                    sb[k][j] += g[j];
+                    sw[k][j] = __builtin_fmaf(g[j], xhat[j], sw[k][j]);
+                }
         }
-        now = next;
-        r = next_r;
-        live = next_live;
+        row_totals<TPR>(s, part[turn]);
+#pragma unroll
+        for (int k = 0; k < K; ++k) now.store_dx(a, k, at[k], r, w[k], s[0] * inv, s[1] * inv, d);
+    };
+    RowPieces<T, K, DROP> even, odd;
+    int64_t r0 = (int64_t)blockIdx.x * RPB;
+    if (r0 < a.rows) {
+        even.load(a, at, row_of<TPR>(r0, a.rows));
+        for (;;) {
+            odd.load(a, at, row_of<TPR>(r0 + step, a.rows));
+            work(even, r0, 0);
+            if ((r0 += step) >= a.rows) break;
+            even.load(a, at, row_of<TPR>(r0 + step, a.rows));
+            work(odd, r0, 1);
+            if ((r0 += step) >= a.rows) break;
+        }
     }
     if constexpr (COLS) {
         if constexpr (TPR < 64) {
@@ -619,32 +636,33 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs 
 }
 
 // Long rows, first launch of the backward pass: a chunk's sums of g and g xhat.
-template <class T, bool DROP>
+template <class T, class P, bool DROP>
 __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_sums(NormArgs a) {
+    constexpr int V = Piece<T>::V, K = CHUNK_PIECES;
     __shared__ float part[2][CHUNK_LANES / 64][2];
     const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
     const int64_t units = a.rows * a.chunks;
     int turn = 0;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x, turn ^= 1) {
         const int64_t r = u / a.chunks;
-        Slot at[CHUNK_PIECES];
+        Slot at[K];
         chunk_slots<T>(at, (int)(u % a.chunks), a.cols);
-        RowPieces<T, CHUNK_PIECES, DROP> now;
-        now.load(a, at, r, true);
-        float s[2] = {0.0f, 0.0f};
+        RowPieces<T, K, DROP> now;
+        now.load(a, at, r);
+        float d[DROP ? K : 1][V], s[2] = {0.0f, 0.0f};
+        now.dropped_share(a, key, at, r, d);
 #pragma unroll
-        for (int k = 0; k < CHUNK_PIECES; ++k) {
-            const u32x4 mask = piece_mask<T>(at[k].skip);
-            now.dy[k].w &= mask;
-            if constexpr (DROP) now.dd[k].w &= mask;
-            float g[Piece<T>::V], p[Piece<T>::V];
-            now.gradient(a, key, at[k], mask, r, k, g);
-            if (a.w) load_params<T>(p, a.w, a.w_is_f32, at[k].c);
+        for (int k = 0; k < K; ++k) {
+            float g[V];
+            Params<T, P> w;
+            if (a.w) w.load(a.w, at[k].c);
+            else w.ones();
+            now.template gradient<true>(k, piece_mask<T>(at[k].skip), at[k].skip, d, g);
 #pragma unroll
-            for (int j = 0; j < Piece<T>::V; ++j) {
-                if (a.w) g[j] *= p[j];
-                s[0] += g[j];
-                s[1] += g[j] * ((floored(now.x[k].at(j), a.relu_floor) - now.mean) * now.rstd);
+            for (int j = 0; j < V; ++j) {
+                const float gw = g[j] * w.at(j);
+                s[0] += gw;
+                s[1] = __builtin_fmaf(gw, now.xhat(a, k, j), s[1]);
             }
         }
         row_totals<CHUNK_LANES>(s, part[turn]);
@@ -653,54 +671,51 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_sums(NormArgs a) {
 }
 
 // Second launch: workgroup (chunk, part) walks the rows part, part + parts, ...: dx of its chunk, and its share of dw and db.
-template <class T, bool DROP, bool COLS>
+template <class T, class P, bool DROP, bool COLS>
 __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_backward(NormArgs a) {
-    constexpr int V = Piece<T>::V;
+    constexpr int V = Piece<T>::V, K = CHUNK_PIECES;
     const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
     const int ch = (int)(blockIdx.x % (unsigned)a.chunks), lane = threadIdx.x & 63;
     const int64_t first = blockIdx.x / (unsigned)a.chunks, step = gridDim.x / (unsigned)a.chunks;
     const float inv = 1.0f / (float)a.cols;
-    Slot at[CHUNK_PIECES];
+    Slot at[K];
     chunk_slots<T>(at, ch, a.cols);
-    float sw[CHUNK_PIECES][V], sb[CHUNK_PIECES][V];
+    float sw[K][V], sb[K][V];
 #pragma unroll
-    for (int k = 0; k < CHUNK_PIECES; ++k)
+    for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int j = 0; j < V; ++j) sw[k][j] = sb[k][j] = 0.0f;
     for (int64_t r = first; r < a.rows; r += step) {
-        RowPieces<T, CHUNK_PIECES, DROP> now;
-        now.load(a, at, r, true);
-        float c1 = 0.0f, c2 = 0.0f;
-        if (a.dx) {
-            for (int i = lane; i < a.chunks; i += 64) {
-                c1 += a.chunk[2 * (r * a.chunks + i)];
-                c2 += a.chunk[2 * (r * a.chunks + i) + 1];
-            }
-            c1 = lanes_total<64>(c1) * inv;
-            c2 = lanes_total<64>(c2) * inv;
+        RowPieces<T, K, DROP> now;
+        now.load(a, at, r);
+        float c1 = 0.0f, c2 = 0.0f, d[DROP ? K : 1][V];
+        for (int i = lane; i < a.chunks; i += 64) {
+            c1 += a.chunk[2 * (r * a.chunks + i)];
+            c2 += a.chunk[2 * (r * a.chunks + i) + 1];
         }
+        c1 = lanes_total<64>(c1) * inv;
+        c2 = lanes_total<64>(c2) * inv;
+        now.dropped_share(a, key, at, r, d);
 #pragma unroll
-        for (int k = 0; k < CHUNK_PIECES; ++k) {
-            const u32x4 mask = piece_mask<T>(at[k].skip);
-            now.dy[k].w &= mask;
-            if constexpr (DROP) now.dd[k].w &= mask;
-            float g[V], p[V];
-            now.gradient(a, key, at[k], mask, r, k, g);
-            if (a.w) load_params<T>(p, a.w, a.w_is_f32, at[k].c);
+        for (int k = 0; k < K; ++k) {
+            Params<T, P> w;
+            if (a.w) w.load(a.w, at[k].c);
+            else w.ones();
+            if (COLS) {
+                float g[V];
+                now.template gradient<true>(k, piece_mask<T>(at[k].skip), at[k].skip, d, g);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if (COLS) {
+                for (int j = 0; j < V; ++j) {
                     sb[k][j] += g[j];
-                    sw[k][j] += g[j] * ((floored(now.x[k].at(j), a.relu_floor) - now.mean) * now.rstd);
+                    sw[k][j] = __builtin_fmaf(g[j], now.xhat(a, k, j), sw[k][j]);
                 }
-                if (a.w) g[j] *= p[j];
             }
-            if (a.dx && at[k].skip < V) store_dx(a, now.x[k], at[k], r, now.mean, now.rstd, c1, c2, g);
+            now.store_dx(a, k, at[k], r, w, c1, c2, d);
         }
     }
     if constexpr (COLS) {
 #pragma unroll
-        for (int k = 0; k < CHUNK_PIECES; ++k) store_cols<V>(a, first, at[k], sw[k], sb[k]);
+        for (int k = 0; k < K; ++k) store_cols<V>(a, first, at[k], sw[k], sb[k]);
     }
 }
 
@@ -727,18 +742,17 @@ __global__ __launch_bounds__(256) void k_norm_backward_narrow(NormArgs a) {
                 g[c] += dropped(a.drop, drop_words(a.drop, key, r, (uint32_t)(c >> 2)).w[c & 3], (float)static_cast<const T*>(a.dd)[r * a.dd_stride + c]);
             const float xhat = (floored(x[c], a.relu_floor) - mean) * rstd;
             sb[c] += g[c];
-            sw[c] += g[c] * xhat;
+            sw[c] = __builtin_fmaf(g[c], xhat, sw[c]);
             if (a.w) g[c] *= param_at<T>(a.w, a.w_is_f32, c);
             c1 += g[c];
-            c2 += g[c] * xhat;
+            c2 = __builtin_fmaf(g[c], xhat, c2);
         }
         c1 *= inv;
         c2 *= inv;
-        if (!a.dx) continue;
 #pragma unroll
         for (int c = 0; c < V; ++c)
             if (c < a.cols) {
-                const float d = rstd * (g[c] - c1 - (floored(x[c], a.relu_floor) - mean) * rstd * c2);
+                const float d = rstd * __builtin_fmaf(-(floored(x[c], a.relu_floor) - mean) * rstd, c2, g[c] - c1);
                 static_cast<T*>(a.dx)[r * a.cols + c] = (T)(x[c] <= a.relu_stop ? 0.0f : d);
             }
     }
@@ -801,13 +815,13 @@ __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
         int64_t r;
         if (BIG) r = i / a.pieces;
         else r = (uint32_t)((((uint64_t)(uint32_t)i * a.magic >> 32) + (uint32_t)i) >> a.shift);
-        const Slot at = slot_at<V>((i - r * a.pieces) * V, a.cols);
-        const Piece<T> q = load_piece(static_cast<const T*>(a.x) + r * a.stride + at.c);
+        const Slot at = slot_at<V>((uint32_t)(i - r * a.pieces) * V, (uint32_t)a.cols);
+        const Piece<T> q = load_piece<T>(static_cast<const T*>(a.x) + r * a.stride, at.c);
         float v[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = q.at(j);
-        if (a.drop.on) drop_piece<T>(a.drop, key, r, at.c, a.cols, v);
-        store_piece(static_cast<T*>(a.y) + r * a.cols + at.c, v);
+        if (a.drop.on) drop_piece<T>(a.drop, key, r, at.c, (uint32_t)a.cols, v);
+        store_piece<T>(static_cast<T*>(a.y) + r * a.cols, at.c, v);
     }
 }
 

@@ -85,15 +85,16 @@ RowShape forward_shape(int32_t type, int64_t cols) {
     if (cols < (type == GNNX_F32 ? 4 : 8)) return {NARROW, 0};
     for (int lanes = 1; lanes <= 64; lanes *= 2)
         if (pieces <= lanes) return {lanes, 1};
-    return pieces <= 128 ? RowShape{64, 2} : pieces <= 256 ? RowShape{64, 4} : pieces <= 512 ? RowShape{256, 2} : pieces <= 1024 ? RowShape{256, 4} :
-           pieces <= 2048 ? RowShape{1024, 2} : RowShape{LONG, 0};
+    for (int lanes : {64, 256})
+        if (pieces <= 4 * lanes) return {lanes, (int)((pieces + lanes - 1) / lanes)};
+    return pieces <= 2048 ? RowShape{1024, 2} : RowShape{LONG, 0};
 }
 RowShape backward_shape(int32_t type, int64_t cols) {
     const int64_t pieces = pieces_of(type, cols);
     if (cols < (type == GNNX_F32 ? 4 : 8)) return {NARROW, 0};
-    for (int lanes = 1; lanes <= 64; lanes *= 2)
+    for (int lanes = 1; lanes <= 1024; lanes *= 2)
         if (pieces <= lanes) return {lanes, 1};
-    return pieces <= 128 ? RowShape{64, 2} : pieces <= 256 ? RowShape{256, 1} : pieces <= 512 ? RowShape{256, 2} : pieces <= 1024 ? RowShape{512, 2} : RowShape{LONG, 0};
+    return {LONG, 0};
 }
 int chunks_of(int32_t type, int64_t cols) {
     const int64_t per = type == GNNX_F32 ? chunk_cols<float>() : chunk_cols<bf16_t>();
@@ -124,66 +125,73 @@ size_t workspace_bytes_of(int32_t type, int64_t rows, int64_t cols, bool backwar
     return b;
 }
 
-template <class T, int TPR, int K, bool DROP>
+template <class T, class P, int TPR, int K, bool DROP>
 void forward_rows(const NormArgs& a, hipStream_t s) {
     constexpr int NT = norm_threads<TPR>();
-    hipLaunchKernelGGL((k_norm_forward<T, TPR, K, DROP>), dim3(grid_of(a.rows, NT / TPR, NT)), dim3(NT), 0, s, a);
+    hipLaunchKernelGGL((k_norm_forward<T, P, TPR, K, DROP>), dim3(grid_of(a.rows, NT / TPR, NT)), dim3(NT), 0, s, a);
 }
 
-template <class T, bool DROP>
+template <class T, class P, bool DROP>
 void run_forward(const NormArgs& a, RowShape sh, hipStream_t s) {
     const unsigned units = grid_of(a.rows * a.chunks, 1, CHUNK_LANES);
     switch (sh.lanes * 8 + sh.pieces) {
-        case 1 * 8 + 1: forward_rows<T, 1, 1, DROP>(a, s); break;
-        case 2 * 8 + 1: forward_rows<T, 2, 1, DROP>(a, s); break;
-        case 4 * 8 + 1: forward_rows<T, 4, 1, DROP>(a, s); break;
-        case 8 * 8 + 1: forward_rows<T, 8, 1, DROP>(a, s); break;
-        case 16 * 8 + 1: forward_rows<T, 16, 1, DROP>(a, s); break;
-        case 32 * 8 + 1: forward_rows<T, 32, 1, DROP>(a, s); break;
-        case 64 * 8 + 1: forward_rows<T, 64, 1, DROP>(a, s); break;
-        case 64 * 8 + 2: forward_rows<T, 64, 2, DROP>(a, s); break;
-        case 64 * 8 + 4: forward_rows<T, 64, 4, DROP>(a, s); break;
-        case 256 * 8 + 2: forward_rows<T, 256, 2, DROP>(a, s); break;
-        case 256 * 8 + 4: forward_rows<T, 256, 4, DROP>(a, s); break;
-        case 1024 * 8 + 2: forward_rows<T, 1024, 2, DROP>(a, s); break;
+        case 1 * 8 + 1: forward_rows<T, P, 1, 1, DROP>(a, s); break;
+        case 2 * 8 + 1: forward_rows<T, P, 2, 1, DROP>(a, s); break;
+        case 4 * 8 + 1: forward_rows<T, P, 4, 1, DROP>(a, s); break;
+        case 8 * 8 + 1: forward_rows<T, P, 8, 1, DROP>(a, s); break;
+        case 16 * 8 + 1: forward_rows<T, P, 16, 1, DROP>(a, s); break;
+        case 32 * 8 + 1: forward_rows<T, P, 32, 1, DROP>(a, s); break;
+        case 64 * 8 + 1: forward_rows<T, P, 64, 1, DROP>(a, s); break;
+        case 64 * 8 + 2: forward_rows<T, P, 64, 2, DROP>(a, s); break;
+        case 64 * 8 + 3: forward_rows<T, P, 64, 3, DROP>(a, s); break;
+        case 64 * 8 + 4: forward_rows<T, P, 64, 4, DROP>(a, s); break;
+        case 256 * 8 + 2: forward_rows<T, P, 256, 2, DROP>(a, s); break;
+        case 256 * 8 + 3: forward_rows<T, P, 256, 3, DROP>(a, s); break;
+        case 256 * 8 + 4: forward_rows<T, P, 256, 4, DROP>(a, s); break;
+        case 1024 * 8 + 2: forward_rows<T, P, 1024, 2, DROP>(a, s); break;
         case NARROW: hipLaunchKernelGGL((k_norm_forward_narrow<T, DROP>), dim3(grid_of(a.rows, 256, 256)), dim3(256), 0, s, a); break;
         default:
             hipLaunchKernelGGL((k_norm_chunk_stats<T>), dim3(units), dim3(CHUNK_LANES), 0, s, a);
-            hipLaunchKernelGGL((k_norm_chunk_outputs<T, DROP>), dim3(units), dim3(CHUNK_LANES), 0, s, a);
+            hipLaunchKernelGGL((k_norm_chunk_outputs<T, P, DROP>), dim3(units), dim3(CHUNK_LANES), 0, s, a);
     }
 }
 
-template <class T, int TPR, int K, bool DROP>
+template <class T, class P, int TPR, int K, bool DROP>
 void backward_rows(const NormArgs& a, hipStream_t s) {
     constexpr int NT = norm_threads<TPR>();
-    if (a.parts) hipLaunchKernelGGL((k_norm_backward<T, TPR, K, DROP, true>), dim3((unsigned)a.parts), dim3(NT), 0, s, a);
-    else if (a.rows) hipLaunchKernelGGL((k_norm_backward<T, TPR, K, DROP, false>), dim3(grid_of(a.rows, NT / TPR, NT)), dim3(NT), 0, s, a);
+    if (a.parts) hipLaunchKernelGGL((k_norm_backward<T, P, TPR, K, DROP, true>), dim3((unsigned)a.parts), dim3(NT), 0, s, a);
+    else if (a.rows) hipLaunchKernelGGL((k_norm_backward<T, P, TPR, K, DROP, false>), dim3(grid_of(a.rows, NT / TPR, NT)), dim3(NT), 0, s, a);
 }
 
-template <class T, bool DROP>
+template <class T, class P, bool DROP>
 void run_backward(const NormArgs& a, RowShape sh, hipStream_t s) {
     switch (sh.lanes * 8 + sh.pieces) {
-        case 1 * 8 + 1: backward_rows<T, 1, 1, DROP>(a, s); break;
-        case 2 * 8 + 1: backward_rows<T, 2, 1, DROP>(a, s); break;
-        case 4 * 8 + 1: backward_rows<T, 4, 1, DROP>(a, s); break;
-        case 8 * 8 + 1: backward_rows<T, 8, 1, DROP>(a, s); break;
-        case 16 * 8 + 1: backward_rows<T, 16, 1, DROP>(a, s); break;
-        case 32 * 8 + 1: backward_rows<T, 32, 1, DROP>(a, s); break;
-        case 64 * 8 + 1: backward_rows<T, 64, 1, DROP>(a, s); break;
-        case 64 * 8 + 2: backward_rows<T, 64, 2, DROP>(a, s); break;
-        case 256 * 8 + 1: backward_rows<T, 256, 1, DROP>(a, s); break;
-        case 256 * 8 + 2: backward_rows<T, 256, 2, DROP>(a, s); break;
-        case 512 * 8 + 2: backward_rows<T, 512, 2, DROP>(a, s); break;
+        case 1 * 8 + 1: backward_rows<T, P, 1, 1, DROP>(a, s); break;
+        case 2 * 8 + 1: backward_rows<T, P, 2, 1, DROP>(a, s); break;
+        case 4 * 8 + 1: backward_rows<T, P, 4, 1, DROP>(a, s); break;
+        case 8 * 8 + 1: backward_rows<T, P, 8, 1, DROP>(a, s); break;
+        case 16 * 8 + 1: backward_rows<T, P, 16, 1, DROP>(a, s); break;
+        case 32 * 8 + 1: backward_rows<T, P, 32, 1, DROP>(a, s); break;
+        case 64 * 8 + 1: backward_rows<T, P, 64, 1, DROP>(a, s); break;
+        case 128 * 8 + 1: backward_rows<T, P, 128, 1, DROP>(a, s); break;
+        case 256 * 8 + 1: backward_rows<T, P, 256, 1, DROP>(a, s); break;
+        case 512 * 8 + 1: backward_rows<T, P, 512, 1, DROP>(a, s); break;
+        case 1024 * 8 + 1: backward_rows<T, P, 1024, 1, DROP>(a, s); break;
         case NARROW: hipLaunchKernelGGL((k_norm_backward_narrow<T, DROP>), dim3(a.parts ? (unsigned)a.parts : grid_of(a.rows, 256, 256)), dim3(256), 0, s, a); break;
         default: {
             const unsigned parts = (unsigned)col_parts(sizeof(T) == 4 ? GNNX_F32 : GNNX_BF16, a.rows, a.cols), grid = (unsigned)a.chunks * parts;
-            if (a.dx && a.rows) hipLaunchKernelGGL((k_norm_chunk_sums<T, DROP>), dim3(grid_of(a.rows * a.chunks, 1, CHUNK_LANES)), dim3(CHUNK_LANES), 0, s, a);
-            if (a.parts) hipLaunchKernelGGL((k_norm_chunk_backward<T, DROP, true>), dim3(grid), dim3(CHUNK_LANES), 0, s, a);
-            else if (a.rows) hipLaunchKernelGGL((k_norm_chunk_backward<T, DROP, false>), dim3(grid), dim3(CHUNK_LANES), 0, s, a);
+            if (a.rows) hipLaunchKernelGGL((k_norm_chunk_sums<T, P, DROP>), dim3(grid_of(a.rows * a.chunks, 1, CHUNK_LANES)), dim3(CHUNK_LANES), 0, s, a);
+            if (a.parts) hipLaunchKernelGGL((k_norm_chunk_backward<T, P, DROP, true>), dim3(grid), dim3(CHUNK_LANES), 0, s, a);
+            else if (a.rows) hipLaunchKernelGGL((k_norm_chunk_backward<T, P, DROP, false>), dim3(grid), dim3(CHUNK_LANES), 0, s, a);
         }
     }
     if (a.parts) hipLaunchKernelGGL((k_norm_join<T>), dim3((unsigned)((2 * a.cols + 31) / 32)), dim3(1024), 0, s, a);
 }
+
+template <class T, class P>
+void forward(const NormArgs& a, RowShape sh, hipStream_t s) { a.d ? run_forward<T, P, true>(a, sh, s) : run_forward<T, P, false>(a, sh, s); }
+template <class T, class P>
+void backward(const NormArgs& a, RowShape sh, hipStream_t s) { a.dd ? run_backward<T, P, true>(a, sh, s) : run_backward<T, P, false>(a, sh, s); }
 
 }  // namespace
 
@@ -207,9 +215,9 @@ extern "C" int gnnx_layer_norm_forward(const gnnx_norm* n, const gnnx_drop* drop
         a.chunks = chunks_of(n->type, a.cols);
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (n->type == GNNX_F32) a.d ? run_forward<float, true>(a, sh, s) : run_forward<float, false>(a, sh, s);
-    else if (n->type == GNNX_BF16) a.d ? run_forward<bf16_t, true>(a, sh, s) : run_forward<bf16_t, false>(a, sh, s);
-    else a.d ? run_forward<f16_t, true>(a, sh, s) : run_forward<f16_t, false>(a, sh, s);
+    if (n->type == GNNX_F32) forward<float, float>(a, sh, s);
+    else if (n->type == GNNX_BF16) a.w_is_f32 ? forward<bf16_t, float>(a, sh, s) : forward<bf16_t, bf16_t>(a, sh, s);
+    else a.w_is_f32 ? forward<f16_t, float>(a, sh, s) : forward<f16_t, f16_t>(a, sh, s);
     return launched("gnnx_layer_norm_forward");
 }
 
@@ -217,9 +225,8 @@ extern "C" int gnnx_layer_norm_backward(const gnnx_norm* n, const gnnx_drop* dro
     NormArgs a;
     if (const char* e = norm_args(n, &a)) return set_error(e);
     if (const char* e = drop_args(drop, &a.drop)) return set_error(e);
-    if (!a.dx && !a.dw && !a.db) return 0;
     if (a.rows > 0 && (a.dd != nullptr) != (drop != nullptr)) return set_error("layer norm: the gradient of a dropped output and its dropout go together");
-    if (a.rows > 0 && ((!a.dy && !a.dd) || !a.x || !a.mean || !a.rstd)) return set_error("null argument");
+    if (a.rows > 0 && ((!a.dy && !a.dd) || !a.x || !a.mean || !a.rstd || !a.dx)) return set_error("null argument");
     const RowShape sh = backward_shape(n->type, a.cols);
     const size_t needed = workspace_bytes_of(n->type, a.rows, a.cols, true);
     if ((a.dw || a.db || sh.lanes == LONG) && (!workspace || workspace_bytes < needed)) return set_error("workspace too small");
@@ -232,9 +239,9 @@ extern "C" int gnnx_layer_norm_backward(const gnnx_norm* n, const gnnx_drop* dro
         a.chunks = chunks_of(n->type, a.cols);
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (n->type == GNNX_F32) a.dd ? run_backward<float, true>(a, sh, s) : run_backward<float, false>(a, sh, s);
-    else if (n->type == GNNX_BF16) a.dd ? run_backward<bf16_t, true>(a, sh, s) : run_backward<bf16_t, false>(a, sh, s);
-    else a.dd ? run_backward<f16_t, true>(a, sh, s) : run_backward<f16_t, false>(a, sh, s);
+    if (n->type == GNNX_F32) backward<float, float>(a, sh, s);
+    else if (n->type == GNNX_BF16) a.w_is_f32 ? backward<bf16_t, float>(a, sh, s) : backward<bf16_t, bf16_t>(a, sh, s);
+    else a.w_is_f32 ? backward<f16_t, float>(a, sh, s) : backward<f16_t, f16_t>(a, sh, s);
     return launched("gnnx_layer_norm_backward");
 }
 
@@ -253,7 +260,7 @@ extern "C" int gnnx_dropout(int32_t type, int64_t rows, int64_t cols, const void
     if (type < 0 || type > 2) return set_error("dropout: type must be 0 (fp32), 1 (bf16) or 2 (fp16)");
     if (!drop) return set_error("null argument");
     if (const char* e = drop_args(drop, &a.drop)) return set_error(e);
-    if (rows < 0 || cols < 0 || x_stride < 0 || cols >= (int64_t(1) << 34)) return set_error("dropout: needs rows, stride >= 0 and 0 <= cols < 2^34");
+    if (rows < 0 || cols < 0 || x_stride < 0 || cols >= (int64_t(1) << 30)) return set_error("dropout: needs rows, stride >= 0 and 0 <= cols < 2^30");
     if (rows == 0 || cols == 0) return 0;
     if (!x || !y) return set_error("null argument");
     a.rows = rows;

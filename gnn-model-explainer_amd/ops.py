@@ -175,14 +175,14 @@ def _norm_backward(dy, dd, x, mean, rstd, weight, relu, drop, need, param_dtype)
     dym, _, _, dys = (None, 0, 0, 0) if dy is None else _rows(dy)
     ddm, _, _, dds = (None, 0, 0, 0) if dd is None else _rows(dd)
     weight, mean, rstd = _param(weight), _param(mean), _param(rstd)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     dw = torch.empty(cols, dtype=param_dtype, device=x.device) if need[1] else None
     db = torch.empty(cols, dtype=param_dtype, device=x.device) if need[2] else None
     ws, nb = _workspace(lib, x, rows, cols, 1) if need[1] or need[2] or cols > _SHORT else (None, 0)
     a = _Norm(_TYPES[x.dtype], int(param_dtype == torch.float32), rows, cols, stride, dys, dds, xm.data_ptr(), _ptr(weight), None, _ptr(dym), _ptr(ddm),
               None, None, _ptr(dx), _ptr(dw), _ptr(db), mean.data_ptr(), rstd.data_ptr(), 0.0, int(bool(relu)))
     _call(x, lib.gnnx_layer_norm_backward, lib, a, d, _ptr(ws), nb)
-    return dx, dw, db
+    return dx if need[0] else None, dw, db
 
 
 class _LayerNorm(torch.autograd.Function):

@@ -446,7 +446,7 @@ typedef struct {
     const void* dd;                         /* backward: gradient of d, or NULL (then no gnnx_drop either) */
     void* y;                                /* forward out, or NULL */
     void* d;                                /* forward out, or NULL (then no gnnx_drop either) */
-    void* dx;                               /* backward out, or NULL */
+    void* dx;                               /* backward out */
     void* dw;                               /* backward out [cols], or NULL */
     void* db;                               /* backward out [cols], or NULL */
     float* mean;                            /* [rows]: forward out (or NULL, with rstd), backward in */
@@ -460,7 +460,7 @@ typedef struct {
 size_t gnnx_layer_norm_workspace_bytes(int32_t type, int64_t rows, int64_t cols, int32_t backward);
 int gnnx_layer_norm_forward(const gnnx_norm* n, const gnnx_drop* drop, void* workspace, size_t workspace_bytes, void* stream);
 int gnnx_layer_norm_backward(const gnnx_norm* n, const gnnx_drop* drop, void* workspace, size_t workspace_bytes, void* stream);
-/* y = dropout(x), y contiguous; its backward pass is the same call on the gradient. */
+/* y = dropout(x), y contiguous, cols < 2^30; its backward pass is the same call on the gradient. */
 int gnnx_dropout(int32_t type, int64_t rows, int64_t cols, const void* x, int64_t x_stride, void* y, const gnnx_drop* drop, void* stream);
 
 const char* gnnx_last_error(void);

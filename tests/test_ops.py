@@ -432,7 +432,7 @@ def test_the_c_entry_points_refuse_what_they_cannot_do(be):
     for n, ws in ((norm(dw=out.data_ptr(), dy=x.data_ptr(), mean=out.data_ptr(), rstd=out.data_ptr()), 0), (norm(dx=out.data_ptr()), 0),
                   (norm(dx=out.data_ptr(), dy=x.data_ptr()), 0), (norm(dx=out.data_ptr(), dd=x.data_ptr(), mean=out.data_ptr(), rstd=out.data_ptr()), 0)):
         assert lib.gnnx_layer_norm_backward(n, None, None, ws, None) != 0
-    for args in ((3, 4, 8), (0, -1, 8), (0, 4, -1), (0, 4, 1 << 34)):
+    for args in ((3, 4, 8), (0, -1, 8), (0, 4, -1), (0, 4, 1 << 30)):
         assert lib.gnnx_dropout(*args, x.data_ptr(), 8, out.data_ptr(), drop, None) != 0
     assert lib.gnnx_dropout(0, 4, 8, None, 8, out.data_ptr(), drop, None) != 0
     assert lib.gnnx_dropout(0, 4, 8, x.data_ptr(), 8, out.data_ptr(), None, None) != 0
