@@ -204,12 +204,14 @@ __device__ __forceinline__ float lanes_total(float v) {
     return v;
 }
 // Sums over the TPR lanes that share a row, in every one of them; beyond a wave through `part` (one float per wave and sum; two calls in a row need two).
+// WHOLE: however many waves the workgroup has.
+constexpr int WHOLE = 1024;
 template <int TPR, int N>
 __device__ __forceinline__ void row_totals(float (&v)[N], float (*part)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = lanes_total<(TPR < 64 ? TPR : 64)>(v[i]);
     if constexpr (TPR > 64) {
-        constexpr int W = TPR / 64;
+        const int W = TPR == WHOLE ? (int)(blockDim.x >> 6) : TPR / 64;
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
             for (int i = 0; i < N; ++i) part[threadIdx.x >> 6][i] = v[i];
@@ -217,7 +219,6 @@ __device__ __forceinline__ void row_totals(float (&v)[N], float (*part)[N]) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float s = 0.0f;
-#pragma unroll
             for (int w = 0; w < W; ++w) s += part[w][i];
             v[i] = s;
         }
@@ -541,7 +542,7 @@ __device__ __forceinline__ void store_cols(const NormArgs& a, int64_t part, cons
 // the wait for the row before it a wait for everything).
 template <class T, class P, int TPR, int K, bool DROP, bool COLS>
 __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs a) {
-    constexpr int V = Piece<T>::V, RPB = norm_threads<TPR>() / TPR;
+    constexpr int V = Piece<T>::V, RPB = norm_threads<TPR>() / TPR;      // (WHOLE: one row, as many waves as hold it)
     __shared__ float part[2][TPR > 64 ? TPR / 64 : 1][2];
     const int l = threadIdx.x % TPR;
     const float inv = 1.0f / (float)a.cols;

@@ -89,12 +89,14 @@ RowShape forward_shape(int32_t type, int64_t cols) {
         if (pieces <= 4 * lanes) return {lanes, (int)((pieces + lanes - 1) / lanes)};
     return pieces <= 2048 ? RowShape{1024, 2} : RowShape{LONG, 0};
 }
+// One piece per lane; rows of more than a wave's pieces take a workgroup of as many waves as hold them.  (Two to four pieces per lane of fewer waves cost registers
+// for the sums of dw and db - 8 to 16 per piece and as many again - and were 2 to 20 % slower at 1024 to 8192 columns.)
 RowShape backward_shape(int32_t type, int64_t cols) {
     const int64_t pieces = pieces_of(type, cols);
     if (cols < (type == GNNX_F32 ? 4 : 8)) return {NARROW, 0};
-    for (int lanes = 1; lanes <= 1024; lanes *= 2)
+    for (int lanes = 1; lanes <= 64; lanes *= 2)
         if (pieces <= lanes) return {lanes, 1};
-    return {LONG, 0};
+    return pieces <= WHOLE ? RowShape{(int)((pieces + 63) / 64) * 64, 1} : RowShape{LONG, 0};
 }
 int chunks_of(int32_t type, int64_t cols) {
     const int64_t per = type == GNNX_F32 ? chunk_cols<float>() : chunk_cols<bf16_t>();
@@ -109,9 +111,12 @@ int col_parts(int32_t type, int64_t rows, int64_t cols) {
         parts = 1024 / chunks_of(type, cols);
         if (parts > rows / 2) parts = rows / 2;
     } else {
-        const int64_t per = sh.lanes == NARROW ? 256 : sh.lanes <= 64 ? 256 / sh.lanes : 1, groups = (rows + per - 1) / per;
+        // 2^17 threads, two waves per SIMD, but a workgroup per CU at least: more waves gain nothing with a row always in flight, and each leaves a partial row to write
+        // and read again (8192 x 8192 bf16: 256 workgroups 87 us, 512: 103, 1024: 124)
+        const int64_t threads = sh.lanes <= 64 ? 256 : sh.lanes, per = sh.lanes == NARROW ? 256 : threads == 256 ? 256 / sh.lanes : 1, groups = (rows + per - 1) / per;
+        const int64_t most = threads > 512 ? 256 : (1 << 17) / threads;
         parts = groups / 2;
-        if (parts > 1024) parts = 1024;
+        if (parts > most) parts = most;
     }
     return (int)(parts < 1 ? 1 : parts);
 }
@@ -156,29 +161,26 @@ void run_forward(const NormArgs& a, RowShape sh, hipStream_t s) {
     }
 }
 
-template <class T, class P, int TPR, int K, bool DROP>
-void backward_rows(const NormArgs& a, hipStream_t s) {
-    constexpr int NT = norm_threads<TPR>();
-    if (a.parts) hipLaunchKernelGGL((k_norm_backward<T, P, TPR, K, DROP, true>), dim3((unsigned)a.parts), dim3(NT), 0, s, a);
-    else if (a.rows) hipLaunchKernelGGL((k_norm_backward<T, P, TPR, K, DROP, false>), dim3(grid_of(a.rows, NT / TPR, NT)), dim3(NT), 0, s, a);
+template <class T, class P, int TPR, bool DROP>
+void backward_rows(const NormArgs& a, int lanes, hipStream_t s) {
+    const int threads = TPR == WHOLE ? lanes : 256, per = TPR == WHOLE ? 1 : 256 / TPR;
+    if (a.parts) hipLaunchKernelGGL((k_norm_backward<T, P, TPR, 1, DROP, true>), dim3((unsigned)a.parts), dim3(threads), 0, s, a);
+    else if (a.rows) hipLaunchKernelGGL((k_norm_backward<T, P, TPR, 1, DROP, false>), dim3(grid_of(a.rows, per, threads)), dim3(threads), 0, s, a);
 }
 
 template <class T, class P, bool DROP>
 void run_backward(const NormArgs& a, RowShape sh, hipStream_t s) {
-    switch (sh.lanes * 8 + sh.pieces) {
-        case 1 * 8 + 1: backward_rows<T, P, 1, 1, DROP>(a, s); break;
-        case 2 * 8 + 1: backward_rows<T, P, 2, 1, DROP>(a, s); break;
-        case 4 * 8 + 1: backward_rows<T, P, 4, 1, DROP>(a, s); break;
-        case 8 * 8 + 1: backward_rows<T, P, 8, 1, DROP>(a, s); break;
-        case 16 * 8 + 1: backward_rows<T, P, 16, 1, DROP>(a, s); break;
-        case 32 * 8 + 1: backward_rows<T, P, 32, 1, DROP>(a, s); break;
-        case 64 * 8 + 1: backward_rows<T, P, 64, 1, DROP>(a, s); break;
-        case 128 * 8 + 1: backward_rows<T, P, 128, 1, DROP>(a, s); break;
-        case 256 * 8 + 1: backward_rows<T, P, 256, 1, DROP>(a, s); break;
-        case 512 * 8 + 1: backward_rows<T, P, 512, 1, DROP>(a, s); break;
-        case 1024 * 8 + 1: backward_rows<T, P, 1024, 1, DROP>(a, s); break;
+    switch (sh.lanes) {
+        case 1: backward_rows<T, P, 1, DROP>(a, 1, s); break;
+        case 2: backward_rows<T, P, 2, DROP>(a, 2, s); break;
+        case 4: backward_rows<T, P, 4, DROP>(a, 4, s); break;
+        case 8: backward_rows<T, P, 8, DROP>(a, 8, s); break;
+        case 16: backward_rows<T, P, 16, DROP>(a, 16, s); break;
+        case 32: backward_rows<T, P, 32, DROP>(a, 32, s); break;
+        case 64: backward_rows<T, P, 64, DROP>(a, 64, s); break;
         case NARROW: hipLaunchKernelGGL((k_norm_backward_narrow<T, DROP>), dim3(a.parts ? (unsigned)a.parts : grid_of(a.rows, 256, 256)), dim3(256), 0, s, a); break;
-        default: {
+        default: backward_rows<T, P, WHOLE, DROP>(a, sh.lanes, s); break;
+        case LONG: {
             const unsigned parts = (unsigned)col_parts(sizeof(T) == 4 ? GNNX_F32 : GNNX_BF16, a.rows, a.cols), grid = (unsigned)a.chunks * parts;
             if (a.rows) hipLaunchKernelGGL((k_norm_chunk_sums<T, P, DROP>), dim3(grid_of(a.rows * a.chunks, 1, CHUNK_LANES)), dim3(CHUNK_LANES), 0, s, a);
             if (a.parts) hipLaunchKernelGGL((k_norm_chunk_backward<T, P, DROP, true>), dim3(grid), dim3(CHUNK_LANES), 0, s, a);
