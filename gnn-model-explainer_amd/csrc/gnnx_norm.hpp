@@ -35,8 +35,7 @@ struct NormArgs {
     void *y, *d, *dx, *dw, *db;
     float *mean, *rstd;
     float eps;
-    float relu_floor;        // v = maximum(x, relu_floor): 0, or -inf without ReLU
-    float relu_stop;         // dx = 0 where x <= relu_stop: 0, or NaN (never) without ReLU
+    float relu_floor;        // v = maximum(x, relu_floor): 0 (then dx = 0 where x <= 0), or -inf without ReLU
     int32_t w_is_f32;        // type of w, b, dw, db: 1 fp32, 0 the type of x
     float* part;             // [parts][2][cols] partial sums of dw and db
     int32_t parts;
@@ -116,9 +115,13 @@ __device__ __forceinline__ void store_piece(void* row, uint32_t c, const float* 
 #pragma unroll
         for (int j = 0; j < 4; ++j) q.w[j] = __builtin_bit_cast(uint32_t, v[j]);
     } else {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef T t2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            q.w[j] = (uint32_t)__builtin_bit_cast(uint16_t, (T)v[2 * j]) | (uint32_t)__builtin_bit_cast(uint16_t, (T)v[2 * j + 1]) << 16;
+        for (int j = 0; j < 4; ++j) {      // two at a time: one conversion instruction per word
+            const f32x2 pair = {v[2 * j], v[2 * j + 1]};
+            q.w[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, t2));
+        }
     }
     __builtin_memcpy(static_cast<char*>(row) + c * (uint32_t)sizeof(T), &q.w, 16);
 }
@@ -199,29 +202,37 @@ __device__ __forceinline__ float lanes_total(float v) {
     if constexpr (TPR > 2) v = lane_pair_sum<2>(v);
     if constexpr (TPR > 4) v = lane_pair_sum<4>(v);
     if constexpr (TPR > 8) v = lane_pair_sum<8>(v);
-    if constexpr (TPR > 16) v = lane_pair_sum<16>(v);
-    if constexpr (TPR > 32) v = lane_pair_sum<32>(v);
+    if constexpr (TPR == 32) v = lane_pair_sum<16>(v);
+    if constexpr (TPR == 64) {      // the four 16-lane sums through scalar registers: no trip through LDS
+        const int i = __builtin_bit_cast(int, v);
+        const float q0 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 0)), q1 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 16));
+        const float q2 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 32)), q3 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 48));
+        v = (q0 + q1) + (q2 + q3);
+    }
     return v;
 }
-// Sums over the TPR lanes that share a row, in every one of them; beyond a wave through `part` (one float per wave and sum; two calls in a row need two).
+// Sums over the TPR lanes that share a row, in every one of them; beyond a wave through `part`, one entry per wave of at most 16 and sum (two calls in a row need
+// two), which the 16 lanes of a DPP row read and add at once.  Entries of waves that the workgroup lacks hold 0: clear_part, before the first call.
 // WHOLE: however many waves the workgroup has.
 constexpr int WHOLE = 1024;
+template <int TPR, int M, int N>
+__device__ __forceinline__ void clear_part(float (&part)[M][16][N]) {
+    if constexpr (TPR > 64) {
+        for (int i = threadIdx.x; i < M * 16 * N; i += (int)blockDim.x) (&part[0][0][0])[i] = 0.0f;
+        __syncthreads();
+    }
+}
 template <int TPR, int N>
 __device__ __forceinline__ void row_totals(float (&v)[N], float (*part)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = lanes_total<(TPR < 64 ? TPR : 64)>(v[i]);
     if constexpr (TPR > 64) {
-        const int W = TPR == WHOLE ? (int)(blockDim.x >> 6) : TPR / 64;
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
             for (int i = 0; i < N; ++i) part[threadIdx.x >> 6][i] = v[i];
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float s = 0.0f;
-            for (int w = 0; w < W; ++w) s += part[w][i];
-            v[i] = s;
-        }
+        for (int i = 0; i < N; ++i) v[i] = lanes_total<16>(part[threadIdx.x & 15][i]);
     }
 }
 
@@ -293,7 +304,8 @@ __device__ __forceinline__ float pieces_squares(const Piece<T> (&q)[K], const Sl
 template <class T, class P, int TPR, int K, bool DROP>
 __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a) {
     constexpr int V = Piece<T>::V, RPB = norm_threads<TPR>() / TPR;
-    __shared__ float part[2][TPR > 64 ? TPR / 64 : 1][1];
+    __shared__ float part[2][16][1];
+    clear_part<TPR>(part);
     const int l = threadIdx.x % TPR;
     const float inv = 1.0f / (float)a.cols;
     const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
@@ -349,7 +361,8 @@ __device__ __forceinline__ void chunk_slots(Slot (&at)[CHUNK_PIECES], int ch, in
 // First launch of the forward pass: the chunk's mean and its sum of squared distances from that mean.
 template <class T>
 __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_stats(NormArgs a) {
-    __shared__ float part[2][CHUNK_LANES / 64][1];
+    __shared__ float part[2][16][1];
+    clear_part<CHUNK_LANES>(part);
     const int64_t units = a.rows * a.chunks;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
         const int64_t r = u / a.chunks;
@@ -509,16 +522,17 @@ struct RowPieces {
             if constexpr (DROP) g[j] += !MASKED || j >= skip ? d[k][j] : 0.0f;
         }
     }
-    // dx of piece k from the row's c1, c2
+    // dx of piece k from the row's rstd c1, rstd c2
     template <class P>
     __device__ __forceinline__ void store_dx(const NormArgs& a, int k, const Slot& at, int64_t r, const Params<T, P>& w, float c1, float c2,
                                              const float (&d)[DROP ? K : 1][V]) const {
         float g[V];
         gradient<false>(k, (u32x4)0u, 0, d, g);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float v = rstd * __builtin_fmaf(-xhat(a, k, j), c2, g[j] * w.at(j) - c1);
-            g[j] = x[k].at(j) <= a.relu_stop ? 0.0f : v;
+        for (int j = 0; j < V; ++j) g[j] = __builtin_fmaf(xhat(a, k, j), -c2, __builtin_fmaf(g[j] * w.at(j), rstd, -c1));
+        if (a.relu_floor == 0.0f) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) g[j] = x[k].at(j) <= 0.0f ? 0.0f : g[j];
         }
         store_piece<T>(static_cast<T*>(a.dx) + r * a.cols, at.c, g);
     }
@@ -543,7 +557,8 @@ __device__ __forceinline__ void store_cols(const NormArgs& a, int64_t part, cons
 template <class T, class P, int TPR, int K, bool DROP, bool COLS>
 __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs a) {
     constexpr int V = Piece<T>::V, RPB = norm_threads<TPR>() / TPR;      // (WHOLE: one row, as many waves as hold it)
-    __shared__ float part[2][TPR > 64 ? TPR / 64 : 1][2];
+    __shared__ float part[2][16][2];
+    clear_part<TPR>(part);
     const int l = threadIdx.x % TPR;
     const float inv = 1.0f / (float)a.cols;
     const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
@@ -585,8 +600,9 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs 
                 }
         }
         row_totals<TPR>(s, part[turn]);
+        const float c1 = s[0] * inv * now.rstd, c2 = s[1] * inv * now.rstd;
 #pragma unroll
-        for (int k = 0; k < K; ++k) now.store_dx(a, k, at[k], r, w[k], s[0] * inv, s[1] * inv, d);
+        for (int k = 0; k < K; ++k) now.store_dx(a, k, at[k], r, w[k], c1, c2, d);
     };
     RowPieces<T, K, DROP> even, odd;
     int64_t r0 = (int64_t)blockIdx.x * RPB;
@@ -640,7 +656,8 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs 
 template <class T, class P, bool DROP>
 __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_sums(NormArgs a) {
     constexpr int V = Piece<T>::V, K = CHUNK_PIECES;
-    __shared__ float part[2][CHUNK_LANES / 64][2];
+    __shared__ float part[2][16][2];
+    clear_part<CHUNK_LANES>(part);
     const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
     const int64_t units = a.rows * a.chunks;
     int turn = 0;
@@ -694,8 +711,8 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_backward(NormArgs a)
             c1 += a.chunk[2 * (r * a.chunks + i)];
             c2 += a.chunk[2 * (r * a.chunks + i) + 1];
         }
-        c1 = lanes_total<64>(c1) * inv;
-        c2 = lanes_total<64>(c2) * inv;
+        c1 = lanes_total<64>(c1) * inv * now.rstd;
+        c2 = lanes_total<64>(c2) * inv * now.rstd;
         now.dropped_share(a, key, at, r, d);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -748,13 +765,13 @@ __global__ __launch_bounds__(256) void k_norm_backward_narrow(NormArgs a) {
             c1 += g[c];
             c2 = __builtin_fmaf(g[c], xhat, c2);
         }
-        c1 *= inv;
-        c2 *= inv;
+        c1 *= inv * rstd;
+        c2 *= inv * rstd;
 #pragma unroll
         for (int c = 0; c < V; ++c)
             if (c < a.cols) {
-                const float d = rstd * __builtin_fmaf(-(floored(x[c], a.relu_floor) - mean) * rstd, c2, g[c] - c1);
-                static_cast<T*>(a.dx)[r * a.cols + c] = (T)(x[c] <= a.relu_stop ? 0.0f : d);
+                const float d = __builtin_fmaf((floored(x[c], a.relu_floor) - mean) * rstd, -c2, __builtin_fmaf(g[c], rstd, -c1));
+                static_cast<T*>(a.dx)[r * a.cols + c] = (T)(a.relu_floor == 0.0f && x[c] <= 0.0f ? 0.0f : d);
             }
     }
     if (!a.parts) return;

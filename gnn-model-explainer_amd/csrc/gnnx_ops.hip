@@ -70,7 +70,6 @@ const char* norm_args(const gnnx_norm* n, NormArgs* a) {
     a->rstd = n->rstd;
     a->eps = n->eps;
     a->relu_floor = n->relu ? 0.0f : -std::numeric_limits<float>::infinity();
-    a->relu_stop = n->relu ? 0.0f : std::numeric_limits<float>::quiet_NaN();
     a->w_is_f32 = n->w_is_f32 != 0 || n->type == GNNX_F32;
     return nullptr;
 }
