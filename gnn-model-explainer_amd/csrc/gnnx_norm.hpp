@@ -46,13 +46,20 @@ struct NormArgs {
 
 struct Philox4 { uint32_t w[4]; };
 
+// a ^ b ^ c in one instruction
+#if defined(__HIPCC__)
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
+#else
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return a ^ b ^ c; }      // (the host compiler of the tests' emulator)
+#endif
+
 // Philox-4x32-10: Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011 (the constants are the paper's).
 __device__ __forceinline__ Philox4 philox(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1) {
 #pragma unroll
     for (int i = 0; i < 10; ++i) {
         const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
-        c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
-        c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+        c0 = xor3((uint32_t)(p1 >> 32), c1, k0);
+        c2 = xor3((uint32_t)(p0 >> 32), c3, k1);
         c1 = (uint32_t)p1;
         c3 = (uint32_t)p0;
         k0 += 0x9E3779B9u;
@@ -72,9 +79,8 @@ __device__ __forceinline__ Philox4 drop_words(const DropArgs& a, const DropKey& 
     const uint64_t row = (uint64_t)(r + a.row0);
     return philox(block, (uint32_t)row, (uint32_t)(row >> 32), k.step, k.k0, k.k1);
 }
-__device__ __forceinline__ float dropped(const DropArgs& a, uint32_t word, float v) {
-    return word > a.last_dropped || !a.on ? v * a.scale : 0.0f;
-}
+__device__ __forceinline__ bool kept(const DropArgs& a, uint32_t word) { return word > a.last_dropped || !a.on; }
+__device__ __forceinline__ float dropped(const DropArgs& a, uint32_t word, float v) { return kept(a, word) ? v * a.scale : 0.0f; }
 
 __device__ __forceinline__ float floored(float v, float floor) { return __builtin_elementwise_maximum(v, floor); }      // ReLU or nothing; NaN stays NaN
 
@@ -147,17 +153,17 @@ __device__ __forceinline__ Slot slot_at(uint32_t c, uint32_t cols) {      // col
     return over <= 0 ? Slot{c, 0} : Slot{cols - V, over < V ? over : V};
 }
 
-// The dropout of a piece's V elements from column c on (c is a multiple of 4 unless the piece was moved back from the end of a row that 4 does not divide:
-// its words then lie across V / 4 + 1 blocks).
+// Which of a piece's V elements from column c on stay (c is a multiple of 4 unless the piece was moved back from the end of a row that 4 does not divide: its words
+// then lie across V / 4 + 1 blocks).  Needs nothing of the data: a kernel forms it while its loads are on their way, a lane mask in scalar registers per element.
 template <class T>
-__device__ __forceinline__ void drop_piece(const DropArgs& d, const DropKey& key, int64_t r, uint32_t c, uint32_t cols, float* v) {
+__device__ __forceinline__ void keep_piece(const DropArgs& d, const DropKey& key, int64_t r, uint32_t c, uint32_t cols, bool* keep) {
     constexpr int V = Piece<T>::V;
     if ((cols & 3) == 0) {
 #pragma unroll
         for (int h = 0; h < V; h += 4) {
             const Philox4 q = drop_words(d, key, r, (c >> 2) + h / 4);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[h + j] = dropped(d, q.w[j], v[h + j]);
+            for (int j = 0; j < 4; ++j) keep[h + j] = kept(d, q.w[j]);
         }
     } else {
         uint32_t w[V + 4];
@@ -172,7 +178,7 @@ __device__ __forceinline__ void drop_piece(const DropArgs& d, const DropKey& key
         for (int j = 0; j < V; ++j) {
             const uint32_t w0 = w[j], w1 = w[j + 1], w2 = w[j + 2], w3 = w[j + 3];      // (values: a choice between the elements would index memory)
             const uint32_t lo = sh & 1 ? w1 : w0, hi = sh & 1 ? w3 : w2;
-            v[j] = dropped(d, sh & 2 ? hi : lo, v[j]);
+            keep[j] = kept(d, sh & 2 ? hi : lo);
         }
     }
 }
@@ -238,7 +244,8 @@ __device__ __forceinline__ void row_totals(float (&v)[N], float (*part)[N]) {
 
 // y (and d) of one piece from its xhat
 template <class T, class P, bool DROP>
-__device__ __forceinline__ void norm_outputs(const NormArgs& a, const DropKey& key, int64_t r, uint32_t c, const Params<T, P>& w, const Params<T, P>& b, float* v) {
+__device__ __forceinline__ void norm_outputs(const NormArgs& a, int64_t r, uint32_t c, const Params<T, P>& w, const Params<T, P>& b,
+                                             const bool* keep, float* v) {
     constexpr int V = Piece<T>::V;
     if (a.w && a.b) {
 #pragma unroll
@@ -252,7 +259,8 @@ __device__ __forceinline__ void norm_outputs(const NormArgs& a, const DropKey& k
     }
     if (a.y) store_piece<T>(static_cast<T*>(a.y) + r * a.cols, c, v);
     if (DROP) {
-        drop_piece<T>(a.drop, key, r, c, (uint32_t)a.cols, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = keep[j] ? v[j] * a.drop.scale : 0.0f;
         store_piece<T>(static_cast<T*>(a.d) + r * a.cols, c, v);
     }
 }
@@ -326,6 +334,10 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
         if (a.b)
 #pragma unroll
             for (int k = 0; k < K; ++k) b[k].load(a.b, at[k].c);
+        bool keep[K][V];
+        if (DROP)
+#pragma unroll
+            for (int k = 0; k < K; ++k) keep_piece<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, keep[k]);
         float s[1] = {pieces_sum(q, at, a.relu_floor)};
         row_totals<TPR>(s, part[0]);
         const float mean = s[0] * inv;
@@ -341,7 +353,7 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
             float v[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) v[j] = (floored(q[k].at(j), a.relu_floor) - mean) * rstd;
-            norm_outputs<T, P, DROP>(a, key, r, at[k].c, w[k], b[k], v);
+            norm_outputs<T, P, DROP>(a, r, at[k].c, w[k], b[k], keep[k], v);
         }
     }
 }
@@ -440,7 +452,9 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_outputs(NormArgs a) 
             Params<T, P> w, b;
             if (a.w) w.load(a.w, at[k].c);
             if (a.b) b.load(a.b, at[k].c);
-            norm_outputs<T, P, DROP>(a, key, r, at[k].c, w, b, v);
+            bool keep[Piece<T>::V];
+            if (DROP) keep_piece<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, keep);
+            norm_outputs<T, P, DROP>(a, r, at[k].c, w, b, keep, v);
         }
     }
 }
@@ -504,9 +518,10 @@ struct RowPieces {
         if constexpr (DROP) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
+                bool keep[V];
+                keep_piece<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, keep);
 #pragma unroll
-                for (int j = 0; j < V; ++j) d[k][j] = dd[k].at(j);
-                drop_piece<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, d[k]);
+                for (int j = 0; j < V; ++j) d[k][j] = keep[j] ? dd[k].at(j) * a.drop.scale : 0.0f;
             }
         }
     }
@@ -836,9 +851,10 @@ __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
         const Slot at = slot_at<V>((uint32_t)(i - r * a.pieces) * V, (uint32_t)a.cols);
         const Piece<T> q = load_piece<T>(static_cast<const T*>(a.x) + r * a.stride, at.c);
         float v[V];
+        bool keep[V];
+        keep_piece<T>(a.drop, key, r, at.c, (uint32_t)a.cols, keep);
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = q.at(j);
-        if (a.drop.on) drop_piece<T>(a.drop, key, r, at.c, (uint32_t)a.cols, v);
+        for (int j = 0; j < V; ++j) v[j] = keep[j] ? q.at(j) * a.drop.scale : 0.0f;
         store_piece<T>(static_cast<T*>(a.y) + r * a.cols, at.c, v);
     }
 }
