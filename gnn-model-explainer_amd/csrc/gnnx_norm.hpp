@@ -359,7 +359,7 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
 }
 
 // ---- rows too long for a workgroup's registers: cut into chunks of CHUNK_LANES x CHUNK_PIECES pieces, a workgroup each, in two launches ----
-constexpr int CHUNK_LANES = 256, CHUNK_PIECES = 4;
+constexpr int CHUNK_LANES = 256, CHUNK_PIECES = 1;
 template <class T>
 constexpr int chunk_cols() { return CHUNK_LANES * CHUNK_PIECES * Piece<T>::V; }
 // the slots of a lane in chunk `ch`; every chunk but a row's last is full
@@ -574,7 +574,7 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs 
     constexpr int V = Piece<T>::V, RPB = norm_threads<TPR>() / TPR;      // (WHOLE: one row, as many waves as hold it)
     __shared__ float part[2][16][2];
     clear_part<TPR>(part);
-    const int l = threadIdx.x % TPR;
+    const int l = threadIdx.x % TPR, lanes = TPR == WHOLE ? (int)blockDim.x : TPR;
     const float inv = 1.0f / (float)a.cols;
     const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
     Slot at[K];
@@ -582,7 +582,7 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_backward(NormArgs 
     float sw[K][V], sb[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        at[k] = slot_at<V>((k * TPR + l) * V, (uint32_t)a.cols);
+        at[k] = slot_at<V>((k * lanes + l) * V, (uint32_t)a.cols);
         if (a.w) w[k].load(a.w, at[k].c);
         else w[k].ones();
 #pragma unroll
@@ -718,23 +718,22 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_backward(NormArgs a)
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int j = 0; j < V; ++j) sw[k][j] = sb[k][j] = 0.0f;
-    for (int64_t r = first; r < a.rows; r += step) {
-        RowPieces<T, K, DROP> now;
-        now.load(a, at, r);
+    Params<T, P> w[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if (a.w) w[k].load(a.w, at[k].c);
+        else w[k].ones();
+    }
+    const auto work = [&](const RowPieces<T, K, DROP>& now, int64_t r) {
         float c1 = 0.0f, c2 = 0.0f, d[DROP ? K : 1][V];
         for (int i = lane; i < a.chunks; i += 64) {
             c1 += a.chunk[2 * (r * a.chunks + i)];
             c2 += a.chunk[2 * (r * a.chunks + i) + 1];
         }
-        c1 = lanes_total<64>(c1) * inv * now.rstd;
-        c2 = lanes_total<64>(c2) * inv * now.rstd;
         now.dropped_share(a, key, at, r, d);
+        if (COLS)
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            Params<T, P> w;
-            if (a.w) w.load(a.w, at[k].c);
-            else w.ones();
-            if (COLS) {
+            for (int k = 0; k < K; ++k) {
                 float g[V];
                 now.template gradient<true>(k, piece_mask<T>(at[k].skip), at[k].skip, d, g);
 #pragma unroll
@@ -743,7 +742,22 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_backward(NormArgs a)
                     sw[k][j] = __builtin_fmaf(g[j], now.xhat(a, k, j), sw[k][j]);
                 }
             }
-            now.store_dx(a, k, at[k], r, w, c1, c2, d);
+        c1 = lanes_total<64>(c1) * inv * now.rstd;
+        c2 = lanes_total<64>(c2) * inv * now.rstd;
+#pragma unroll
+        for (int k = 0; k < K; ++k) now.store_dx(a, k, at[k], r, w[k], c1, c2, d);
+    };
+    RowPieces<T, K, DROP> even, odd;
+    int64_t r = first;
+    if (r < a.rows) {
+        even.load(a, at, r);
+        for (;;) {
+            odd.load(a, at, r + step < a.rows ? r + step : r);
+            work(even, r);
+            if ((r += step) >= a.rows) break;
+            even.load(a, at, r + step < a.rows ? r + step : r);
+            work(odd, r);
+            if ((r += step) >= a.rows) break;
         }
     }
     if constexpr (COLS) {

@@ -95,7 +95,8 @@ RowShape backward_shape(int32_t type, int64_t cols) {
     if (cols < (type == GNNX_F32 ? 4 : 8)) return {NARROW, 0};
     for (int lanes = 1; lanes <= 64; lanes *= 2)
         if (pieces <= lanes) return {lanes, 1};
-    return pieces <= WHOLE ? RowShape{(int)((pieces + 63) / 64) * 64, 1} : RowShape{LONG, 0};
+    if (pieces <= WHOLE) return {(int)((pieces + 63) / 64) * 64, 1};
+    return type == GNNX_F32 && pieces <= 2 * WHOLE ? RowShape{(int)((pieces + 127) / 128) * 64, 2} : RowShape{LONG, 0};
 }
 int chunks_of(int32_t type, int64_t cols) {
     const int64_t per = type == GNNX_F32 ? chunk_cols<float>() : chunk_cols<bf16_t>();
@@ -107,7 +108,7 @@ int col_parts(int32_t type, int64_t rows, int64_t cols) {
     const RowShape sh = backward_shape(type, cols);
     int64_t parts;
     if (sh.lanes == LONG) {
-        parts = 1024 / chunks_of(type, cols);
+        parts = 512 / chunks_of(type, cols);
         if (parts > rows / 2) parts = rows / 2;
     } else {
         // 2^17 threads, two waves per SIMD, but a workgroup per CU at least: more waves gain nothing with a row always in flight, and each leaves a partial row to write
@@ -160,11 +161,11 @@ void run_forward(const NormArgs& a, RowShape sh, hipStream_t s) {
     }
 }
 
-template <class T, class P, int TPR, bool DROP>
+template <class T, class P, int TPR, bool DROP, int K = 1>
 void backward_rows(const NormArgs& a, int lanes, hipStream_t s) {
     const int threads = TPR == WHOLE ? lanes : 256, per = TPR == WHOLE ? 1 : 256 / TPR;
-    if (a.parts) hipLaunchKernelGGL((k_norm_backward<T, P, TPR, 1, DROP, true>), dim3((unsigned)a.parts), dim3(threads), 0, s, a);
-    else if (a.rows) hipLaunchKernelGGL((k_norm_backward<T, P, TPR, 1, DROP, false>), dim3(grid_of(a.rows, per, threads)), dim3(threads), 0, s, a);
+    if (a.parts) hipLaunchKernelGGL((k_norm_backward<T, P, TPR, K, DROP, true>), dim3((unsigned)a.parts), dim3(threads), 0, s, a);
+    else if (a.rows) hipLaunchKernelGGL((k_norm_backward<T, P, TPR, K, DROP, false>), dim3(grid_of(a.rows, per, threads)), dim3(threads), 0, s, a);
 }
 
 template <class T, class P, bool DROP>
@@ -178,7 +179,15 @@ void run_backward(const NormArgs& a, RowShape sh, hipStream_t s) {
         case 32: backward_rows<T, P, 32, DROP>(a, 32, s); break;
         case 64: backward_rows<T, P, 64, DROP>(a, 64, s); break;
         case NARROW: hipLaunchKernelGGL((k_norm_backward_narrow<T, DROP>), dim3(a.parts ? (unsigned)a.parts : grid_of(a.rows, 256, 256)), dim3(256), 0, s, a); break;
-        default: backward_rows<T, P, WHOLE, DROP>(a, sh.lanes, s); break;
+        default:
+            if constexpr (sizeof(T) == 4) {
+                if (sh.pieces == 2) {
+                    backward_rows<T, P, WHOLE, DROP, 2>(a, sh.lanes, s);
+                    break;
+                }
+            }
+            backward_rows<T, P, WHOLE, DROP>(a, sh.lanes, s);
+            break;
         case LONG: {
             const unsigned parts = (unsigned)col_parts(sizeof(T) == 4 ? GNNX_F32 : GNNX_BF16, a.rows, a.cols), grid = (unsigned)a.chunks * parts;
             if (a.rows) hipLaunchKernelGGL((k_norm_chunk_sums<T, P, DROP>), dim3(grid_of(a.rows * a.chunks, 1, CHUNK_LANES)), dim3(CHUNK_LANES), 0, s, a);
