@@ -820,22 +820,33 @@ __global__ __launch_bounds__(256) void k_norm_backward_narrow(NormArgs a) {
     }
 }
 
-// The partial sums of a column: 32 columns and 32 parts at a time per workgroup, each of the 32 sums in part order, then the 32 in order.
-template <class T>
-__global__ __launch_bounds__(1024) void k_norm_join(NormArgs a) {
-    __shared__ float sums[32][33];
-    const int64_t i = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31), n = 2 * a.cols;      // dw's columns, then db's
+// The partial sums of a column in part order.  MANY: 32 columns and 32 parts at a time per workgroup (each of the 32 sums in part order, then the 32 in order), else
+// a thread per column - rows so long that they left few partial rows: 7 of 65537 columns 10 us with MANY, 3 without.
+template <class T, bool MANY>
+__global__ __launch_bounds__(MANY ? 1024 : 256) void k_norm_join(NormArgs a) {
+    const int64_t n = 2 * a.cols;      // dw's columns, then db's
+    int64_t i;
     float s = 0.0f;
-    if (i < n) {
+    if constexpr (MANY) {
+        __shared__ float sums[32][33];
+        i = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+        if (i < n) {
 #pragma unroll 8
-        for (int p = threadIdx.x >> 5; p < a.parts; p += 32) s += a.part[(int64_t)p * n + i];
-    }
-    sums[threadIdx.x >> 5][threadIdx.x & 31] = s;
-    __syncthreads();
-    if (threadIdx.x >= 32 || i >= n) return;
-    s = 0.0f;
+            for (int p = threadIdx.x >> 5; p < a.parts; p += 32) s += a.part[(int64_t)p * n + i];
+        }
+        sums[threadIdx.x >> 5][threadIdx.x & 31] = s;
+        __syncthreads();
+        if (threadIdx.x >= 32) return;
+        s = 0.0f;
 #pragma unroll
-    for (int p = 0; p < 32; ++p) s += sums[p][threadIdx.x];
+        for (int p = 0; p < 32; ++p) s += sums[p][threadIdx.x];
+        if (i >= n) return;
+    } else {
+        i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+        if (i >= n) return;
+#pragma unroll 8
+        for (int p = 0; p < a.parts; ++p) s += a.part[(int64_t)p * n + i];
+    }
     void* out = i >= a.cols ? a.db : a.dw;
     const int64_t c = i >= a.cols ? i - a.cols : i;
     if (!out) return;

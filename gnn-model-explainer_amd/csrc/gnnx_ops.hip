@@ -195,7 +195,8 @@ void run_backward(const NormArgs& a, RowShape sh, hipStream_t s) {
             else if (a.rows) hipLaunchKernelGGL((k_norm_chunk_backward<T, P, DROP, false>), dim3(grid), dim3(CHUNK_LANES), 0, s, a);
         }
     }
-    if (a.parts) hipLaunchKernelGGL((k_norm_join<T>), dim3((unsigned)((2 * a.cols + 31) / 32)), dim3(1024), 0, s, a);
+    if (a.parts > 16) hipLaunchKernelGGL((k_norm_join<T, true>), dim3((unsigned)((2 * a.cols + 31) / 32)), dim3(1024), 0, s, a);
+    else if (a.parts) hipLaunchKernelGGL((k_norm_join<T, false>), dim3((unsigned)((2 * a.cols + 255) / 256)), dim3(256), 0, s, a);
 }
 
 template <class T, class P>
