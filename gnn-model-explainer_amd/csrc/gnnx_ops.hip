@@ -111,10 +111,11 @@ int col_parts(int32_t type, int64_t rows, int64_t cols) {
         parts = 512 / chunks_of(type, cols);
         if (parts > rows / 2) parts = rows / 2;
     } else {
-        // 2^17 threads, two waves per SIMD, but a workgroup per CU at least: more waves gain nothing with a row always in flight, and each leaves a partial row to write
-        // and read again (8192 x 8192 bf16: 256 workgroups 87 us, 512: 103, 1024: 124)
-        const int64_t threads = sh.lanes <= 64 ? 256 : sh.lanes, per = sh.lanes == NARROW ? 256 : threads == 256 ? 256 / sh.lanes : 1, groups = (rows + per - 1) / per;
-        const int64_t most = threads > 512 ? 256 : (1 << 17) / threads;
+        // Eight waves per CU, in whole workgroups per CU (2.67 of three waves each left a third of the CUs with more to do than the rest: 20011 x 1280 bf16 44 us, 4: 39):
+        // more waves gain nothing with a row always in flight, and each workgroup leaves a partial row to write and read again (8192 x 8192 bf16: 256 workgroups
+        // 87 us, 512: 103, 1024: 124; 99997 x 20 fp32: 128 15.6 us, 256 11.1, 512 10.1).
+        const int64_t threads = sh.lanes <= 64 ? 256 : sh.lanes, per = sh.lanes == NARROW ? 256 : sh.lanes <= 64 ? 256 / sh.lanes : 1, groups = (rows + per - 1) / per;
+        const int64_t most = 256 * ((512 + threads - 1) / threads);
         parts = groups / 2;
         if (parts > most) parts = most;
     }
