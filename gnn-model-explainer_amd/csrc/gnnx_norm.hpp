@@ -84,6 +84,13 @@ __device__ __forceinline__ float dropped(const DropArgs& a, uint32_t word, float
 
 __device__ __forceinline__ float floored(float v, float floor) { return __builtin_elementwise_maximum(v, floor); }      // ReLU or nothing; NaN stays NaN
 
+// (variance + eps)^-1/2: the hardware's reciprocal square root (within one ulp), its argument kept out of the subnormal numbers it takes for 0
+__device__ __forceinline__ float reciprocal_deviation(float v) {
+    const bool tiny = v < 0x1p-96f;
+    const float y = __builtin_amdgcn_rsqf(tiny ? v * 0x1p96f : v);
+    return tiny ? y * 0x1p48f : y;
+}
+
 template <class T>
 __device__ __forceinline__ float param_at(const void* p, int32_t is_f32, int64_t c) {
     return is_f32 ? static_cast<const float*>(p)[c] : (float)static_cast<const T*>(p)[c];
@@ -140,9 +147,11 @@ struct Params {
 #pragma unroll
         for (int i = 0; i < N; ++i) q[i] = load_piece<P>(p, c + i * Piece<P>::V);
     }
-    __device__ __forceinline__ void ones() {
+    __device__ __forceinline__ void ones() { fill(sizeof(P) == 4 ? 0x3f800000u : __is_same(P, bf16_t) ? 0x3f803f80u : 0x3c003c00u); }
+    __device__ __forceinline__ void zeros() { fill(0u); }
+    __device__ __forceinline__ void fill(uint32_t v) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) q[i].w = (u32x4)(sizeof(P) == 4 ? 0x3f800000u : __is_same(P, bf16_t) ? 0x3f803f80u : 0x3c003c00u);
+        for (int i = 0; i < N; ++i) q[i].w = (u32x4)v;
     }
     __device__ __forceinline__ float at(int j) const { return q[j / Piece<P>::V].at(j % Piece<P>::V); }
 };
@@ -247,16 +256,8 @@ template <class T, class P, bool DROP>
 __device__ __forceinline__ void norm_outputs(const NormArgs& a, int64_t r, uint32_t c, const Params<T, P>& w, const Params<T, P>& b,
                                              const bool* keep, float* v) {
     constexpr int V = Piece<T>::V;
-    if (a.w && a.b) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = __builtin_fmaf(v[j], w.at(j), b.at(j));
-    } else if (a.w) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] *= w.at(j);
-    } else if (a.b) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] += b.at(j);
-    }
+    for (int j = 0; j < V; ++j) v[j] = __builtin_fmaf(v[j], w.at(j), b.at(j));
     if (a.y) store_piece<T>(static_cast<T*>(a.y) + r * a.cols, c, v);
     if (DROP) {
 #pragma unroll
@@ -283,20 +284,21 @@ __device__ __forceinline__ int64_t row_of(int64_t r0, int64_t rows) {
 template <int TPR>
 constexpr int norm_threads() { return TPR <= 64 ? 256 : TPR; }
 
-// sum of a lane's K pieces (first the mean's), and of their squared distances from `mean`: the elements that another piece has as well are left out
-template <class T, int K>
+// sum of a lane's K pieces, and of their squared distances from `mean`; FULL: every element of every piece counts (the row is TPR K V long), else those that another
+// piece has as well are left out
+template <bool FULL, class T, int K>
 __device__ __forceinline__ float pieces_sum(const Piece<T> (&q)[K], const Slot (&at)[K], float floor) {
     float s = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         Piece<T> p = q[k];
-        if (k + 1 == K) p.w &= piece_mask<T>(at[k].skip);
+        if (!FULL && k + 1 == K) p.w &= piece_mask<T>(at[k].skip);
 #pragma unroll
         for (int j = 0; j < Piece<T>::V; ++j) s += floored(p.at(j), floor);
     }
     return s;
 }
-template <class T, int K>
+template <bool FULL, class T, int K>
 __device__ __forceinline__ float pieces_squares(const Piece<T> (&q)[K], const Slot (&at)[K], float floor, float mean) {
     float s = 0.0f;
 #pragma unroll
@@ -304,7 +306,7 @@ __device__ __forceinline__ float pieces_squares(const Piece<T> (&q)[K], const Sl
 #pragma unroll
         for (int j = 0; j < Piece<T>::V; ++j) {
             const float v = floored(q[k].at(j), floor) - mean;
-            s = k + 1 < K || j >= at[k].skip ? __builtin_fmaf(v, v, s) : s;
+            s = FULL || k + 1 < K || j >= at[k].skip ? __builtin_fmaf(v, v, s) : s;
         }
     return s;
 }
@@ -315,6 +317,7 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
     __shared__ float part[2][16][1];
     clear_part<TPR>(part);
     const int l = threadIdx.x % TPR;
+    const bool full = a.cols == TPR * K * V;
     const float inv = 1.0f / (float)a.cols;
     const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
@@ -328,22 +331,26 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
             at[k] = slot_at<V>((k * TPR + l) * V, (uint32_t)a.cols);
             q[k] = load_piece<T>(x, at[k].c);
         }
-        if (a.w)
 #pragma unroll
-            for (int k = 0; k < K; ++k) w[k].load(a.w, at[k].c);
-        if (a.b)
-#pragma unroll
-            for (int k = 0; k < K; ++k) b[k].load(a.b, at[k].c);
+        for (int k = 0; k < K; ++k) {
+            if (a.w) w[k].load(a.w, at[k].c);
+            else w[k].ones();
+            if (a.b) b[k].load(a.b, at[k].c);
+            else b[k].zeros();
+        }
         bool keep[K][V];
         if (DROP)
 #pragma unroll
             for (int k = 0; k < K; ++k) keep_piece<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, keep[k]);
-        float s[1] = {pieces_sum(q, at, a.relu_floor)};
+        float s[1];
+        if (full) s[0] = pieces_sum<true>(q, at, a.relu_floor);
+        else s[0] = pieces_sum<false>(q, at, a.relu_floor);
         row_totals<TPR>(s, part[0]);
         const float mean = s[0] * inv;
-        s[0] = pieces_squares(q, at, a.relu_floor, mean);
+        if (full) s[0] = pieces_squares<true>(q, at, a.relu_floor, mean);
+        else s[0] = pieces_squares<false>(q, at, a.relu_floor, mean);
         row_totals<TPR>(s, part[1]);
-        const float rstd = 1.0f / sqrtf(s[0] * inv + a.eps);
+        const float rstd = reciprocal_deviation(s[0] * inv + a.eps);
         if (l == 0 && a.mean) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
@@ -439,7 +446,7 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_outputs(NormArgs a) 
             const float d = st[2 * i] - mean;
             s += st[2 * i + 1] + d * d * (float)(left < chunk_cols<T>() ? left : chunk_cols<T>());
         }
-        const float rstd = 1.0f / sqrtf(lanes_total<64>(s) / (float)a.cols + a.eps);
+        const float rstd = reciprocal_deviation(lanes_total<64>(s) / (float)a.cols + a.eps);
         if (ch == 0 && threadIdx.x == 0 && a.mean) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
@@ -451,7 +458,9 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_outputs(NormArgs a) 
             for (int j = 0; j < Piece<T>::V; ++j) v[j] = (floored(q[k].at(j), a.relu_floor) - mean) * rstd;
             Params<T, P> w, b;
             if (a.w) w.load(a.w, at[k].c);
+            else w.ones();
             if (a.b) b.load(a.b, at[k].c);
+            else b.zeros();
             bool keep[Piece<T>::V];
             if (DROP) keep_piece<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, keep);
             norm_outputs<T, P, DROP>(a, r, at[k].c, w, b, keep, v);
@@ -474,7 +483,7 @@ __global__ __launch_bounds__(256) void k_norm_forward_narrow(NormArgs a) {
             const float v = floored((float)x[c], a.relu_floor) - mean;
             s = __builtin_fmaf(v, v, s);
         }
-        const float rstd = 1.0f / sqrtf(s * inv + a.eps);
+        const float rstd = reciprocal_deviation(s * inv + a.eps);
         if (a.mean) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;

@@ -84,6 +84,7 @@ inline int emu_update_dpp(int old, int src, int ctrl, int row_mask, int bank_mas
 inline float emu_fmed3f(float a, float b, float c) { return std::fmax(std::fmin(a, b), std::fmin(std::fmax(a, b), c)); }
 #define __builtin_amdgcn_fmed3f(a, b, c) emu_fmed3f((a), (b), (c))
 #define __builtin_amdgcn_sqrtf(x) emu::hw_form(std::sqrt(x))
+#define __builtin_amdgcn_rsqf(x) emu::hw_form(1.0f / std::sqrt(x))
 #define __expf(x) emu::hw_form(std::exp(x))
 inline float atomicAdd(float* p, float v) { float o = *p; *p = o + v; return o; }
 inline unsigned atomicOr(unsigned* p, unsigned v) { unsigned o = *p; *p = o | v; return o; }
