@@ -68,6 +68,11 @@ __device__ __forceinline__ Philox4 philox(uint32_t c0, uint32_t c1, uint32_t c2,
     return {{c0, c1, c2, c3}};
 }
 
+// The value is needed here (no instruction): what it is computed from may not move behind.
+#ifndef GNNX_OPAQUE
+#define GNNX_OPAQUE(x) asm volatile("" : "+v"(x))
+#endif
+
 struct DropKey { uint32_t k0, k1, step; };
 __device__ __forceinline__ DropKey drop_key(const DropArgs& a) {
     if (!a.state) return {a.k0, a.k1, a.step};
@@ -162,17 +167,18 @@ __device__ __forceinline__ Slot slot_at(uint32_t c, uint32_t cols) {      // col
     return over <= 0 ? Slot{c, 0} : Slot{cols - V, over < V ? over : V};
 }
 
-// Which of a piece's V elements from column c on stay (c is a multiple of 4 unless the piece was moved back from the end of a row that 4 does not divide: its words
-// then lie across V / 4 + 1 blocks).  Needs nothing of the data: a kernel forms it while its loads are on their way, a lane mask in scalar registers per element.
+// The words of a piece's V elements from column c on (c is a multiple of 4 unless the piece was moved back from the end of a row that 4 does not divide: its words
+// then lie across V / 4 + 1 blocks).  They need nothing of the data: a kernel forms them while its loads are on their way, and compares them where it needs the
+// answer (truth values held that long are packed into bytes by the compiler, at 6 instructions each).
 template <class T>
-__device__ __forceinline__ void keep_piece(const DropArgs& d, const DropKey& key, int64_t r, uint32_t c, uint32_t cols, bool* keep) {
+__device__ __forceinline__ void piece_words(const DropArgs& d, const DropKey& key, int64_t r, uint32_t c, uint32_t cols, uint32_t* out) {
     constexpr int V = Piece<T>::V;
     if ((cols & 3) == 0) {
 #pragma unroll
         for (int h = 0; h < V; h += 4) {
             const Philox4 q = drop_words(d, key, r, (c >> 2) + h / 4);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) keep[h + j] = kept(d, q.w[j]);
+            for (int j = 0; j < 4; ++j) out[h + j] = q.w[j];
         }
     } else {
         uint32_t w[V + 4];
@@ -187,7 +193,7 @@ __device__ __forceinline__ void keep_piece(const DropArgs& d, const DropKey& key
         for (int j = 0; j < V; ++j) {
             const uint32_t w0 = w[j], w1 = w[j + 1], w2 = w[j + 2], w3 = w[j + 3];      // (values: a choice between the elements would index memory)
             const uint32_t lo = sh & 1 ? w1 : w0, hi = sh & 1 ? w3 : w2;
-            keep[j] = kept(d, sh & 2 ? hi : lo);
+            out[j] = sh & 2 ? hi : lo;
         }
     }
 }
@@ -254,14 +260,14 @@ __device__ __forceinline__ void row_totals(float (&v)[N], float (*part)[N]) {
 // y (and d) of one piece from its xhat
 template <class T, class P, bool DROP>
 __device__ __forceinline__ void norm_outputs(const NormArgs& a, int64_t r, uint32_t c, const Params<T, P>& w, const Params<T, P>& b,
-                                             const bool* keep, float* v) {
+                                             const uint32_t* words, float* v) {
     constexpr int V = Piece<T>::V;
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = __builtin_fmaf(v[j], w.at(j), b.at(j));
     if (a.y) store_piece<T>(static_cast<T*>(a.y) + r * a.cols, c, v);
     if (DROP) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = keep[j] ? v[j] * a.drop.scale : 0.0f;
+        for (int j = 0; j < V; ++j) v[j] = dropped(a.drop, words[j], v[j]);
         store_piece<T>(static_cast<T*>(a.d) + r * a.cols, c, v);
     }
 }
@@ -338,10 +344,14 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
             if (a.b) b[k].load(a.b, at[k].c);
             else b[k].zeros();
         }
-        bool keep[K][V];
+        uint32_t words[K][V];
         if (DROP)
 #pragma unroll
-            for (int k = 0; k < K; ++k) keep_piece<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, keep[k]);
+            for (int k = 0; k < K; ++k) {
+                piece_words<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, words[k]);
+#pragma unroll
+                for (int j = 0; j < V; ++j) GNNX_OPAQUE(words[k][j]);      // before the wait for the row: left alone they move behind the reductions
+            }
         float s[1];
         if (full) s[0] = pieces_sum<true>(q, at, a.relu_floor);
         else s[0] = pieces_sum<false>(q, at, a.relu_floor);
@@ -360,7 +370,7 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
             float v[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) v[j] = (floored(q[k].at(j), a.relu_floor) - mean) * rstd;
-            norm_outputs<T, P, DROP>(a, r, at[k].c, w[k], b[k], keep[k], v);
+            norm_outputs<T, P, DROP>(a, r, at[k].c, w[k], b[k], words[k], v);
         }
     }
 }
@@ -461,9 +471,9 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_outputs(NormArgs a) 
             else w.ones();
             if (a.b) b.load(a.b, at[k].c);
             else b.zeros();
-            bool keep[Piece<T>::V];
-            if (DROP) keep_piece<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, keep);
-            norm_outputs<T, P, DROP>(a, r, at[k].c, w, b, keep, v);
+            uint32_t words[Piece<T>::V];
+            if (DROP) piece_words<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, words);
+            norm_outputs<T, P, DROP>(a, r, at[k].c, w, b, words, v);
         }
     }
 }
@@ -527,10 +537,10 @@ struct RowPieces {
         if constexpr (DROP) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                bool keep[V];
-                keep_piece<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, keep);
+                uint32_t words[V];
+                piece_words<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, words);
 #pragma unroll
-                for (int j = 0; j < V; ++j) d[k][j] = keep[j] ? dd[k].at(j) * a.drop.scale : 0.0f;
+                for (int j = 0; j < V; ++j) d[k][j] = dropped(a.drop, words[j], dd[k].at(j));
             }
         }
     }
@@ -885,10 +895,10 @@ __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
         const Slot at = slot_at<V>((uint32_t)(i - r * a.pieces) * V, (uint32_t)a.cols);
         const Piece<T> q = load_piece<T>(static_cast<const T*>(a.x) + r * a.stride, at.c);
         float v[V];
-        bool keep[V];
-        keep_piece<T>(a.drop, key, r, at.c, (uint32_t)a.cols, keep);
+        uint32_t words[V];
+        piece_words<T>(a.drop, key, r, at.c, (uint32_t)a.cols, words);
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = keep[j] ? q.at(j) * a.drop.scale : 0.0f;
+        for (int j = 0; j < V; ++j) v[j] = dropped(a.drop, words[j], q.at(j));
         store_piece<T>(static_cast<T*>(a.y) + r * a.cols, at.c, v);
     }
 }
