@@ -317,6 +317,11 @@ __device__ __forceinline__ float pieces_squares(const Piece<T> (&q)[K], const Sl
     return s;
 }
 
+// The forward pass: one read of x, mean and then the squared distances from it out of the registers (no E[v^2] - mean^2), one write of each output.
+// Bound by HBM: 65536 x 1024 fp32 90 us = 5.98 TB/s, bf16 (fp32 parameters) 45 us = 5.96, 16384 x 4096 bf16 41 us = 6.6 - a copy reaches 6.1.  One row per group of
+// lanes and no walk over rows: a grid that covers all rows at once streams better than workgroups that stride (copies: 6.1 against 4.4 to 5.6 TB/s).  With a second,
+// dropped output the generator's 40 instructions per four elements fill what the loads leave (65536 x 1024 bf16: 75 us, 93 % of the VALU's issue slots before the
+// words were compared in place, fp32 137 us = 5.9 TB/s).
 template <class T, class P, int TPR, int K, bool DROP>
 __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a) {
     constexpr int V = Piece<T>::V, RPB = norm_threads<TPR>() / TPR;
@@ -387,6 +392,8 @@ __device__ __forceinline__ void chunk_slots(Slot (&at)[CHUNK_PIECES], int ch, in
         at[k] = slot_at<Piece<T>::V>((uint32_t)ch * chunk_cols<T>() + (k * CHUNK_LANES + threadIdx.x) * Piece<T>::V, (uint32_t)cols);
 }
 
+// x is read twice (forward) and x, dy twice (backward), the second time from the caches where they hold it; a workgroup per row left most of the chip idle and read
+// the row three times (48 x 65537 fp32, both passes: 787 us; in chunks 32).  A long row's two statistics are 8 bytes per chunk.
 // First launch of the forward pass: the chunk's mean and its sum of squared distances from that mean.
 template <class T>
 __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_stats(NormArgs a) {
@@ -586,6 +593,8 @@ __device__ __forceinline__ void store_cols(const NormArgs& a, int64_t part, cons
 
 // The backward pass of rows in registers: one pass over x, dy (and dd), dx out.  COLS: a workgroup walks rows a grid apart and keeps its share of dw and db in
 // registers; at the end the lanes that hold the same column add up (lane sums, then LDS across the waves) and the workgroup leaves one partial row of each.
+// Bound by HBM at fp32 (65536 x 1024: 150 us = 5.4 TB/s of x, dy and dx), at 16 bits by HBM and 170 instructions per piece together (83 us = 4.8 TB/s, a 42 % busy
+// VALU, with 5 us of it the join of the partial rows).
 // The next row is always on its way while one is worked on (the last one is loaded again at the end: a load that may or may not have been issued would make
 // the wait for the row before it a wait for everything).
 template <class T, class P, int TPR, int K, bool DROP, bool COLS>
@@ -839,7 +848,7 @@ __global__ __launch_bounds__(256) void k_norm_backward_narrow(NormArgs a) {
     }
 }
 
-// The partial sums of a column in part order.  MANY: 32 columns and 32 parts at a time per workgroup (each of the 32 sums in part order, then the 32 in order), else
+// The partial sums of a column in part order.  MANY: 32 columns and 32 parts at a time per workgroup (each of the 32 sums in part order, then the 32 in four groups), else
 // a thread per column - rows so long that they left few partial rows: 7 of 65537 columns 10 us with MANY, 3 without.
 template <class T, bool MANY>
 __global__ __launch_bounds__(MANY ? 1024 : 256) void k_norm_join(NormArgs a) {
@@ -856,9 +865,10 @@ __global__ __launch_bounds__(MANY ? 1024 : 256) void k_norm_join(NormArgs a) {
         sums[threadIdx.x >> 5][threadIdx.x & 31] = s;
         __syncthreads();
         if (threadIdx.x >= 32) return;
-        s = 0.0f;
+        float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int p = 0; p < 32; ++p) s += sums[p][threadIdx.x];
+        for (int p = 0; p < 32; ++p) q[p & 3] += sums[p][threadIdx.x];
+        s = (q[0] + q[1]) + (q[2] + q[3]);
         if (i >= n) return;
     } else {
         i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -882,7 +892,9 @@ struct DropoutArgs {
     DropArgs drop;
 };
 
-// One thread per piece of a row.  BIG: more pieces in all than 32 bits count.
+// One thread per piece of a row, the words formed before the load returns.  Bound by HBM: 16384 x 4096 bf16 41 us = 6.5 TB/s, 65536 x 1024 fp32 88 us = 6.1 (a copy:
+// 6.1); at 16 bits the generator's 10 instructions per element are close behind (63 % of the VALU's issue slots).  32 bits per element and 10 rounds cost nothing over
+// 16 bits or 7 rounds there.  BIG: more pieces in all than 32 bits count.
 template <class T, bool BIG>
 __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
     constexpr int V = Piece<T>::V;

@@ -108,7 +108,7 @@ int col_parts(int32_t type, int64_t rows, int64_t cols) {
     const RowShape sh = backward_shape(type, cols);
     int64_t parts;
     if (sh.lanes == LONG) {
-        parts = 512 / chunks_of(type, cols);
+        parts = 512 / chunks_of(type, cols);      // two workgroups per CU; 1024: 48 x 65537 fp32 21.1 us for 20.4, 4096 x 16384 bf16 136 for 138
         if (parts > rows / 2) parts = rows / 2;
     } else {
         // Eight waves per CU, in whole workgroups per CU (2.67 of three waves each left a third of the CUs with more to do than the rest: 20011 x 1280 bf16 44 us, 4: 39):
@@ -162,11 +162,15 @@ void run_forward(const NormArgs& a, RowShape sh, hipStream_t s) {
     }
 }
 
+template <class T>
+constexpr int type_code() { return sizeof(T) == 4 ? GNNX_F32 : GNNX_BF16; }      // (fp16 and bf16 have one geometry)
+
+// (without dw and db the walk over the rows is the same: the next row's load needs rows to come)
 template <class T, class P, int TPR, bool DROP, int K = 1>
 void backward_rows(const NormArgs& a, int lanes, hipStream_t s) {
-    const int threads = TPR == WHOLE ? lanes : 256, per = TPR == WHOLE ? 1 : 256 / TPR;
+    const int threads = TPR == WHOLE ? lanes : 256;
     if (a.parts) hipLaunchKernelGGL((k_norm_backward<T, P, TPR, K, DROP, true>), dim3((unsigned)a.parts), dim3(threads), 0, s, a);
-    else if (a.rows) hipLaunchKernelGGL((k_norm_backward<T, P, TPR, K, DROP, false>), dim3(grid_of(a.rows, per, threads)), dim3(threads), 0, s, a);
+    else if (a.rows) hipLaunchKernelGGL((k_norm_backward<T, P, TPR, K, DROP, false>), dim3((unsigned)col_parts(type_code<T>(), a.rows, a.cols)), dim3(threads), 0, s, a);
 }
 
 template <class T, class P, bool DROP>
@@ -190,7 +194,7 @@ void run_backward(const NormArgs& a, RowShape sh, hipStream_t s) {
             backward_rows<T, P, WHOLE, DROP>(a, sh.lanes, s);
             break;
         case LONG: {
-            const unsigned parts = (unsigned)col_parts(sizeof(T) == 4 ? GNNX_F32 : GNNX_BF16, a.rows, a.cols), grid = (unsigned)a.chunks * parts;
+            const unsigned parts = (unsigned)col_parts(type_code<T>(), a.rows, a.cols), grid = (unsigned)a.chunks * parts;
             if (a.rows) hipLaunchKernelGGL((k_norm_chunk_sums<T, P, DROP>), dim3(grid_of(a.rows * a.chunks, 1, CHUNK_LANES)), dim3(CHUNK_LANES), 0, s, a);
             if (a.parts) hipLaunchKernelGGL((k_norm_chunk_backward<T, P, DROP, true>), dim3(grid), dim3(CHUNK_LANES), 0, s, a);
             else if (a.rows) hipLaunchKernelGGL((k_norm_chunk_backward<T, P, DROP, false>), dim3(grid), dim3(CHUNK_LANES), 0, s, a);
