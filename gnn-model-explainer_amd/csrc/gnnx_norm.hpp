@@ -752,9 +752,25 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_backward(NormArgs a)
         if (a.w) w[k].load(a.w, at[k].c);
         else w[k].ones();
     }
-    const auto work = [&](const RowPieces<T, K, DROP>& now, int64_t r) {
-        float c1 = 0.0f, c2 = 0.0f, d[DROP ? K : 1][V];
-        for (int i = lane; i < a.chunks; i += 64) {
+    // the row's sums are on their way with its pieces, two chunks a lane; more chunks (rows of more than 128) when the row is worked on
+    struct Sums { float g[2], x[2]; };
+    const auto sums_of = [&](int64_t r) {
+        Sums q;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int i = lane + 64 * h < a.chunks ? lane + 64 * h : a.chunks - 1;
+            q.g[h] = a.chunk[2 * (r * a.chunks + i)];
+            q.x[h] = a.chunk[2 * (r * a.chunks + i) + 1];
+        }
+        return q;
+    };
+    const auto work = [&](const RowPieces<T, K, DROP>& now, const Sums& q, int64_t r) {
+        float c1 = lane < a.chunks ? q.g[0] : 0.0f, c2 = lane < a.chunks ? q.x[0] : 0.0f, d[DROP ? K : 1][V];
+        if (lane + 64 < a.chunks) {
+            c1 += q.g[1];
+            c2 += q.x[1];
+        }
+        for (int i = lane + 128; i < a.chunks; i += 64) {
             c1 += a.chunk[2 * (r * a.chunks + i)];
             c2 += a.chunk[2 * (r * a.chunks + i) + 1];
         }
@@ -776,15 +792,19 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_backward(NormArgs a)
         for (int k = 0; k < K; ++k) now.store_dx(a, k, at[k], r, w[k], c1, c2, d);
     };
     RowPieces<T, K, DROP> even, odd;
+    Sums even_sums, odd_sums;
     int64_t r = first;
     if (r < a.rows) {
         even.load(a, at, r);
+        even_sums = sums_of(r);
         for (;;) {
             odd.load(a, at, r + step < a.rows ? r + step : r);
-            work(even, r);
+            odd_sums = sums_of(r + step < a.rows ? r + step : r);
+            work(even, even_sums, r);
             if ((r += step) >= a.rows) break;
             even.load(a, at, r + step < a.rows ? r + step : r);
-            work(odd, r);
+            even_sums = sums_of(r + step < a.rows ? r + step : r);
+            work(odd, odd_sums, r);
             if ((r += step) >= a.rows) break;
         }
     }

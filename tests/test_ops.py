@@ -143,7 +143,7 @@ def make(be, rows, cols, dtype, wtype, pad=0, seed=0, params=("w", "b")):
 
 
 SHAPES = [(1, 1), (1, 7), (3, 8), (5, 20), (70, 20), (33, 33), (4, 64), (3, 257), (2, 1000), (5, 1283), (2, 2049), (1, 4100), (2, 4133)]
-BIG = [(1, 8192), (3, 8193), (17, 16385), (2, 32769), (2, 65537), (1, 131073), (9, 4096), (1000, 60), (4099, 20), (300, 513), (40000, 3), (513, 2048), (33, 4095)]
+BIG = [(1, 8192), (3, 8193), (17, 16385), (2, 32769), (2, 65537), (1, 131073), (5, 300007), (9, 4096), (1000, 60), (4099, 20), (300, 513), (40000, 3), (513, 2048), (33, 4095)]
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 
 
