@@ -39,7 +39,8 @@ class LayerNorm(nn.Module):
 
 
 class CounterDropout(nn.Module):
-    """Dropout whose mask is a function of (seed, use, layer, row, feature): ops.dropout.  `uses` counts the calls in training mode."""
+    """Dropout whose mask is a function of (seed, use, layer, row, feature): ops.dropout.  `uses` counts the calls in training mode on the host; a step captured into a
+    graph repeats the use it was captured with (ops.dropout takes a seed tensor for new masks at every replay)."""
 
     def __init__(self, p, seed, layer, layers):
         super().__init__()
