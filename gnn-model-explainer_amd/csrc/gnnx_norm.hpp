@@ -257,17 +257,16 @@ __device__ __forceinline__ void row_totals(float (&v)[N], float (*part)[N]) {
     }
 }
 
-// y (and d) of one piece from its xhat
-template <class T, class P, bool DROP>
-__device__ __forceinline__ void norm_outputs(const NormArgs& a, int64_t r, uint32_t c, const Params<T, P>& w, const Params<T, P>& b,
-                                             const uint32_t* words, float* v) {
+// y (and d) of one piece from its xhat; keep(j): whether element j stays
+template <class T, class P, bool DROP, class Keep>
+__device__ __forceinline__ void norm_outputs(const NormArgs& a, int64_t r, uint32_t c, const Params<T, P>& w, const Params<T, P>& b, const Keep& keep, float* v) {
     constexpr int V = Piece<T>::V;
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = __builtin_fmaf(v[j], w.at(j), b.at(j));
     if (a.y) store_piece<T>(static_cast<T*>(a.y) + r * a.cols, c, v);
     if (DROP) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = dropped(a.drop, words[j], v[j]);
+        for (int j = 0; j < V; ++j) v[j] = keep(j) ? v[j] * a.drop.scale : 0.0f;
         store_piece<T>(static_cast<T*>(a.d) + r * a.cols, c, v);
     }
 }
@@ -350,12 +349,18 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
             else b[k].zeros();
         }
         uint32_t words[K][V];
+        bool flags[V];
         if (DROP)
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 piece_words<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, words[k]);
 #pragma unroll
-                for (int j = 0; j < V; ++j) GNNX_OPAQUE(words[k][j]);      // before the wait for the row: left alone they move behind the reductions
+                for (int j = 0; j < V; ++j) {
+                    // one piece: lane masks in scalar registers (65536 x 512 bf16 43 us for 50 with words); more: the words - either way before the wait for the row,
+                    // which they move behind if left alone
+                    if constexpr (K == 1) flags[j] = kept(a.drop, words[k][j]);
+                    else GNNX_OPAQUE(words[k][j]);
+                }
             }
         float s[1];
         if (full) s[0] = pieces_sum<true>(q, at, a.relu_floor);
@@ -375,7 +380,7 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
             float v[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) v[j] = (floored(q[k].at(j), a.relu_floor) - mean) * rstd;
-            norm_outputs<T, P, DROP>(a, r, at[k].c, w[k], b[k], words[k], v);
+            norm_outputs<T, P, DROP>(a, r, at[k].c, w[k], b[k], [&](int j) { return K == 1 ? flags[j] : kept(a.drop, words[k][j]); }, v);
         }
     }
 }
@@ -480,12 +485,12 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_outputs(NormArgs a) 
             else b.zeros();
             uint32_t words[Piece<T>::V];
             if (DROP) piece_words<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, words);
-            norm_outputs<T, P, DROP>(a, r, at[k].c, w, b, words, v);
+            norm_outputs<T, P, DROP>(a, r, at[k].c, w, b, [&](int j) { return kept(a.drop, words[j]); }, v);
         }
     }
 }
 
-// Rows shorter than one piece (fewer than 4 or 8 columns): one thread per row.
+// Rows shorter than one piece (fewer than 4 or 8 columns): one thread per row, element by element (10^6 x 7 bf16: 22 us = 1.3 TB/s, bound by the 2-byte accesses).
 template <class T, bool DROP>
 __global__ __launch_bounds__(256) void k_norm_forward_narrow(NormArgs a) {
     const float inv = 1.0f / (float)a.cols;
@@ -505,12 +510,19 @@ __global__ __launch_bounds__(256) void k_norm_forward_narrow(NormArgs a) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
         }
-        for (int c = 0; c < a.cols; ++c) {
-            float v = (floored((float)x[c], a.relu_floor) - mean) * rstd;
-            const float w = a.w ? param_at<T>(a.w, a.w_is_f32, c) : 1.0f;
-            v = a.b ? __builtin_fmaf(v, w, param_at<T>(a.b, a.w_is_f32, c)) : v * w;
-            if (a.y) static_cast<T*>(a.y)[r * a.cols + c] = (T)v;
-            if (DROP) static_cast<T*>(a.d)[r * a.cols + c] = (T)dropped(a.drop, drop_words(a.drop, key, r, (uint32_t)(c >> 2)).w[c & 3], v);
+        for (int h = 0; h < a.cols; h += 4) {
+            Philox4 q = {};
+            if (DROP) q = drop_words(a.drop, key, r, (uint32_t)(h >> 2));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = h + j;
+                if (c >= a.cols) break;
+                float v = (floored((float)x[c], a.relu_floor) - mean) * rstd;
+                const float w = a.w ? param_at<T>(a.w, a.w_is_f32, c) : 1.0f;
+                v = a.b ? __builtin_fmaf(v, w, param_at<T>(a.b, a.w_is_f32, c)) : v * w;
+                if (a.y) static_cast<T*>(a.y)[r * a.cols + c] = (T)v;
+                if (DROP) static_cast<T*>(a.d)[r * a.cols + c] = (T)dropped(a.drop, q.w[j], v);
+            }
         }
     }
 }

@@ -35,7 +35,7 @@ def build(force=False):
         objs, running = [], []
         for u in units:      # side by side; the flags are one set for all
             objs.append(os.path.join(HERE, "_build", os.path.basename(u) + ".%d.o" % os.getpid()))
-            cmd = [cxx, "-O2", "-g", "-std=c++17", "-fPIC", "-ffp-contract=on", "-Wno-psabi", "-I", os.path.join(HERE, "include"), "-x", "c++", "-c", u,
+            cmd = [cxx, "-O2", "-g", "-std=c++17", "-fPIC", "-ffp-contract=on", "-Wno-psabi", "-Wno-pass-failed", "-I", os.path.join(HERE, "include"), "-x", "c++", "-c", u,
                    "-o", objs[-1]]
             running.append((cmd, subprocess.Popen(cmd)))
         for cmd, proc in running:
