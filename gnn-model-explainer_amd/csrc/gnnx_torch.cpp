@@ -93,6 +93,13 @@ int type_of(const Tensor& x) {
     }
 }
 
+// forward-mode derivatives would be lost without a word
+void no_tangent(const char* name, const Tensor& t) {
+    if (!t._fw_grad(/*level=*/0).defined()) return;
+    PyErr_SetString(PyExc_NotImplementedError, text(name, " carries a forward-mode derivative, which the operators do not propagate").c_str());
+    throw py::error_already_set();
+}
+
 Tensor input(const char* name, const py::object& o) {
     if (!THPVariable_Check(o.ptr()) || type_of(THPVariable_Unpack(o.ptr())) < 0)
         throw py::type_error(text(name, " must be a float32, bfloat16 or float16 tensor, got ",
@@ -101,6 +108,7 @@ Tensor input(const char* name, const py::object& o) {
     if (x.dim() < 1) throw py::value_error(text(name, " needs at least one dimension"));
     if (g_lib.host ? !x.is_cpu() : !x.is_cuda()) throw std::runtime_error(text("the operators run on MI355X only (no CPU fallback): got a tensor on ", x.device()));
     if (x.layout() != at::kStrided) throw py::type_error(text(name, " must be a dense tensor"));
+    no_tangent(name, x);
     return x;
 }
 
@@ -112,6 +120,7 @@ Tensor parameter(const char* name, const py::object& o, const Tensor& x) {
         throw py::type_error(text(name, " must be float32 or of x's type ", x.scalar_type(), ", got ", p.scalar_type()));
     if (p.dim() != 1 || p.size(0) != x.size(-1)) throw py::value_error(text(name, " must have shape (", x.size(-1), ",), got ", p.sizes()));
     if (p.device() != x.device()) throw py::value_error(text(name, " is on ", p.device(), ", x on ", x.device()));
+    no_tangent(name, p);
     return p;
 }
 

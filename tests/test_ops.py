@@ -429,6 +429,19 @@ def test_refusals(be):
             ops.dropout(x, 0.5, state)
 
 
+def test_forward_mode_derivatives_and_batched_tensors_are_refused(be):
+    import torch.autograd.forward_ad as fwd
+    x, w = torch.randn(4, 8, device=be.device), torch.ones(8, device=be.device)
+    with fwd.dual_level():
+        for call in (lambda: ops.layer_norm(fwd.make_dual(x, x)), lambda: ops.layer_norm(x, fwd.make_dual(w, w)), lambda: ops.dropout(fwd.make_dual(x, x), 0.5, 1)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda v: ops.layer_norm(v, w))(x)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda v: ops.layer_norm(v, w).sum())(x)
+
+
 def test_tensors_off_the_gpu_are_refused():
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ops.dropout(torch.ones(2, 2), 0.5, 1)
