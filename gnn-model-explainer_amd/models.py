@@ -10,7 +10,8 @@ route of the explainer (explainer/torch_route.py) differentiates through for the
 Two options the reference does not have, both read from `args`, both on the kernels of ops.py where the model is on the GPU:
   layer_norm    True: a learned LayerNorm after the ReLU of every hidden layer in the place of apply_bn (state_dict keys norms.<layer>.weight / .bias);
   dropout_seed  an int: the layers' dropout draws its masks from (seed, use, layer, node, feature) instead of torch's generator, so that a training run or an
-                explanation through the torch route is reproducible by itself; `reset_dropout()` starts the uses again.
+                explanation through the torch route is reproducible by itself; `reset_dropout()` starts the uses again, `forward(..., dropout_use=n)` draws the
+                n-th use's whatever ran before (what a forward pass that is run again, as by torch.utils.checkpoint, needs).
 """
 import torch
 import torch.nn as nn
@@ -33,26 +34,33 @@ class LayerNorm(nn.Module):
             return ops.layer_norm(x, self.weight, self.bias, self.eps, relu=True)
         return F.layer_norm(F.relu(x), (self.dim,), self.weight, self.bias, self.eps)
 
-    def with_dropout(self, x, drop):
-        """(self(x), drop(self(x))) in one pass each way (ops.layer_norm_dropout)."""
-        return ops.layer_norm_dropout(x, self.weight, self.bias, drop.p, drop.seed, drop.next_step(), self.eps, relu=True)
+    def with_dropout(self, x, drop, use=None):
+        """(self(x), drop(self(x), use)) in one pass each way (ops.layer_norm_dropout)."""
+        return ops.layer_norm_dropout(x, self.weight, self.bias, drop.p, drop.seed, drop.step(use), self.eps, relu=True)
 
 
 class CounterDropout(nn.Module):
-    """Dropout whose mask is a function of (seed, use, layer, row, feature): ops.dropout.  `uses` counts the calls in training mode on the host; a step captured into a
-    graph repeats the use it was captured with (ops.dropout takes a seed tensor for new masks at every replay)."""
+    """Dropout whose mask is a function of (seed, use, layer, row, feature): ops.dropout.  `use` is the caller's number of this forward pass; left out, `uses` counts the
+    calls in training mode on the host.  A forward pass that is run again must draw the masks it drew first, which a count of calls cannot know: inside a backward pass
+    (recomputation, torch.utils.checkpoint) the use has to be given.  A step captured into a graph repeats the use it was captured with (ops.dropout takes a seed
+    tensor for new masks at every replay)."""
 
     def __init__(self, p, seed, layer, layers):
         super().__init__()
         self.p, self.seed, self.layer, self.layers, self.uses = float(p), int(seed), layer, layers, 0
 
-    def next_step(self):
-        step = self.uses * self.layers + self.layer
-        self.uses += 1
-        return step
+    def step(self, use=None):
+        """The generator's step of the given use, or of the next one."""
+        if use is None:
+            if torch._C._current_graph_task_id() != -1:
+                raise RuntimeError("dropout drawn by a count of its calls, inside a backward pass: a recomputed forward pass would draw other masks than the first one; "
+                                   "pass the number of the training step, dropout_use= to the encoder (use= to CounterDropout), in both")
+            use = self.uses
+            self.uses += 1
+        return use * self.layers + self.layer
 
-    def forward(self, x):
-        return ops.dropout(x, self.p, self.seed, self.next_step()) if self.training else x
+    def forward(self, x, use=None):
+        return ops.dropout(x, self.p, self.seed, self.step(use)) if self.training else x
 
 
 class GraphConv(nn.Module):
@@ -144,22 +152,24 @@ class GcnEncoderGraph(nn.Module):
             if isinstance(m, CounterDropout):
                 m.uses = 0
 
-    def _activate(self, layer, x, nxt):
+    def _activate(self, layer, x, nxt, use):
         """What follows graph convolution `layer` (models.py:239-253): (the layer's embedding, what convolution `nxt` reads, whether that has been through its
         dropout)."""
+        drop = nxt.counter_dropout()
         if self.norms is not None:
-            drop = nxt.counter_dropout()
             if drop is not None:
-                h, d = self.norms[layer].with_dropout(x, drop)
+                h, d = self.norms[layer].with_dropout(x, drop, use)
                 return h, d, True
             x = self.norms[layer](x)
             return x, x, False
         x = self.act(x)
         if self.bn:
             x = self.apply_bn(x)
+        if drop is not None:
+            return x, drop(x, use), True
         return x, x, False
 
-    def _layers(self, x, adj):
+    def _layers(self, x, adj, dropout_use=None):
         """The graph convolutions one after the other: (embedding, attention adjacency) of each."""
         convs = [self.conv_first, *self.conv_block, self.conv_last]
         dropped = False
@@ -168,22 +178,22 @@ class GcnEncoderGraph(nn.Module):
             if i + 1 == len(convs):
                 yield x, adj_att
                 return
-            h, x, dropped = self._activate(i, x, convs[i + 1])
+            h, x, dropped = self._activate(i, x, convs[i + 1], dropout_use)
             yield h, adj_att
 
-    def gcn_forward(self, x, adj):
+    def gcn_forward(self, x, adj, dropout_use=None):
         """models.py:230-267: all layers, concatenated embeddings [1, n, H (L - 1) + O] and the stacked attention adjacencies (the
         block layers re-append conv_first's, as the reference does at :252)."""
         x_all, att_all = [], []
-        for i, (h, adj_att) in enumerate(self._layers(x, adj)):
+        for i, (h, adj_att) in enumerate(self._layers(x, adj, dropout_use)):
             x_all.append(h)
             att_all.append(att_all[0] if 0 < i <= len(self.conv_block) else adj_att)
         return torch.cat(x_all, dim=2), torch.stack(att_all, dim=3)
 
-    def forward(self, x, adj, batch_num_nodes=None, **kwargs):
-        """models.py:269-316: per-layer max over all rows, concat, linear head."""
+    def forward(self, x, adj, batch_num_nodes=None, dropout_use=None, **kwargs):
+        """models.py:269-316: per-layer max over all rows, concat, linear head.  dropout_use: CounterDropout's use."""
         outs, atts = [], []
-        for h, adj_att in self._layers(x, adj):
+        for h, adj_att in self._layers(x, adj, dropout_use):
             outs.append(h.max(dim=1)[0])
             atts.append(adj_att)
         output = torch.cat(outs, dim=1) if self.concat else outs[-1]
@@ -191,7 +201,7 @@ class GcnEncoderGraph(nn.Module):
 
 
 class GcnEncoderNode(GcnEncoderGraph):
-    def forward(self, x, adj, batch_num_nodes=None, **kwargs):
-        """models.py:363-376: the head on every row."""
-        emb, adj_att = self.gcn_forward(x, adj)
+    def forward(self, x, adj, batch_num_nodes=None, dropout_use=None, **kwargs):
+        """models.py:363-376: the head on every row.  dropout_use: CounterDropout's use."""
+        emb, adj_att = self.gcn_forward(x, adj, dropout_use)
         return self.pred_model(emb), adj_att

@@ -627,6 +627,44 @@ def test_command_line_options():
     assert a.layer_norm is False and a.dropout_seed is None
 
 
+@pytest.mark.parametrize("reentrant", [False, True])
+@pytest.mark.parametrize("layer_norm", [False, True])
+def test_a_recomputed_forward_pass_draws_the_masks_it_drew_first(be, layer_norm, reentrant):
+    """torch.utils.checkpoint runs the forward pass again inside the backward pass: with the use given the gradients are those without it, bit for bit; by the count of
+    calls it would draw other masks, and is refused."""
+    from torch.utils.checkpoint import checkpoint
+    g = torch.Generator().manual_seed(16)
+    adj = (torch.rand(2, 12, 12, generator=g) < 0.4).float().to(be.device)
+    x0, up = torch.randn(2, 12, 7, generator=g).to(be.device), torch.randn(2, 12, 3, generator=g).to(be.device)
+    def grads(how):
+        torch.manual_seed(3)
+        args = argparse.Namespace(method="base", bias=True, layer_norm=layer_norm, dropout_seed=9)
+        m = models.GcnEncoderNode(7, 20, 20, 3, 4, bn=False, dropout=0.4, args=args).to(be.device).train()
+        x, kw = x0.clone().requires_grad_(), {} if how == "counted" else {"dropout_use": 5}
+        f = lambda x, adj: m(x, adj, **kw)[0]
+        out = f(x, adj) if how == "plain" else checkpoint(f, x, adj, use_reentrant=reentrant)
+        out.backward(up)
+        return [out.detach(), x.grad] + [p.grad for p in m.parameters()]
+    want, got = grads("plain"), grads("checkpoint")
+    assert all(torch.equal(a, b) for a, b in zip(want, got)) and bool((want[1] != 0).any())
+    with pytest.raises(RuntimeError, match="dropout_use"):
+        grads("counted")
+
+
+def test_the_use_of_an_encoders_dropout_can_be_given(be):
+    """dropout_use=n draws what the n-th counted pass draws and leaves the count alone."""
+    m = _encoder(models.GcnEncoderNode).to(be.device).train()
+    x, adj = torch.randn(1, 6, 7, generator=torch.Generator().manual_seed(1)).to(be.device), torch.ones(1, 6, 6, device=be.device)
+    with torch.no_grad():
+        counted = [m(x, adj)[0] for _ in range(3)]
+        assert all(torch.equal(m(x, adj, dropout_use=i)[0], counted[i]) for i in (2, 0, 1)) and not torch.equal(counted[0], counted[1])
+        assert torch.equal(m(x, adj)[0], m(x, adj, dropout_use=3)[0])
+        m.eval()
+        assert torch.equal(m(x, adj, dropout_use=3)[0], m(x, adj)[0])
+    with pytest.raises(ValueError, match="step"):
+        m.train()(x, adj, dropout_use=-1)
+
+
 # ---------------------------------------------------------------- hardware only ----------------------------------------------------------------
 @pytest.mark.gpu
 def test_captured_training_step_draws_new_masks_at_every_replay():
