@@ -41,7 +41,7 @@ class LayerNorm(nn.Module):
 
 class CounterDropout(nn.Module):
     """Dropout whose mask is a function of (seed, use, layer, row, feature): ops.dropout.  `use` is the caller's number of this forward pass; left out, `uses` counts the
-    calls in training mode on the host.  A forward pass that is run again must draw the masks it drew first, which a count of calls cannot know: inside a backward pass
+    calls in training mode on the host and is part of the state_dict: a training run that is resumed goes on with the masks that come next.  A forward pass that is run again must draw the masks it drew first, which a count of calls cannot know: inside a backward pass
     (recomputation, torch.utils.checkpoint) the use has to be given.  A step captured into a graph repeats the use it was captured with (ops.dropout takes a seed
     tensor for new masks at every replay)."""
 
@@ -58,6 +58,16 @@ class CounterDropout(nn.Module):
             use = self.uses
             self.uses += 1
         return use * self.layers + self.layer
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        destination[prefix + "uses"] = torch.tensor(self.uses)
+
+    def _load_from_state_dict(self, state_dict, prefix, *rest):
+        uses = state_dict.pop(prefix + "uses", None)      # (a state_dict from an encoder without such dropout has none: the count stays)
+        if uses is not None:
+            self.uses = int(uses)
+        super()._load_from_state_dict(state_dict, prefix, *rest)
 
     def forward(self, x, use=None):
         return ops.dropout(x, self.p, self.seed, self.step(use)) if self.training else x
@@ -84,6 +94,11 @@ class GraphConv(nn.Module):
         """The layer's CounterDropout where it is to be applied now, else None."""
         drop = self.dropout_layer if self.dropout > 0.001 else None
         return drop if isinstance(drop, CounterDropout) and drop.training else None
+
+    def _load_from_state_dict(self, state_dict, prefix, *rest):
+        if not isinstance(getattr(self, "dropout_layer", None), CounterDropout):
+            state_dict.pop(prefix + "dropout_layer.uses", None)      # the count of another encoder's CounterDropout
+        super()._load_from_state_dict(state_dict, prefix, *rest)
 
     def forward(self, x, adj, dropped=False):
         """dropped: x has been through this layer's dropout already (LayerNorm.with_dropout)."""

@@ -665,6 +665,29 @@ def test_the_use_of_an_encoders_dropout_can_be_given(be):
         m.train()(x, adj, dropout_use=-1)
 
 
+def test_a_resumed_training_run_goes_on_with_the_next_masks(be, tmp_path):
+    """The count of uses travels with the state_dict; encoders with and without seeded dropout load one another's."""
+    x, adj = torch.randn(1, 6, 7, generator=torch.Generator().manual_seed(1)).to(be.device), torch.ones(1, 6, 6, device=be.device)
+    m = _encoder(models.GcnEncoderNode).to(be.device).train()
+    with torch.no_grad():
+        m(x, adj), m(x, adj)
+        torch.save(m.state_dict(), tmp_path / "mid_run.pth")
+        third = m(x, adj)[0]
+        state = torch.load(tmp_path / "mid_run.pth", weights_only=True)
+        resumed = _encoder(models.GcnEncoderNode).to(be.device).train()
+        assert not resumed.load_state_dict(state).missing_keys
+        assert torch.equal(resumed(x, adj)[0], third) and not torch.equal(resumed(x, adj)[0], third)
+    # an encoder without seeded dropout: its state_dict loads and leaves the count, and it loads one with a count
+    for p in (0.0, 0.4):
+        other = models.GcnEncoderNode(7, 20, 20, 3, 4, bn=False, dropout=p, args=argparse.Namespace(method="base", bias=True, layer_norm=True))
+        assert not any(k.endswith("uses") for k in other.state_dict())
+        other.load_state_dict(state)
+        resumed.load_state_dict(other.state_dict())
+        assert [c.dropout_layer.uses for c in resumed.conv_block] == [4, 4]
+    with pytest.raises(RuntimeError, match="nonsense"):
+        resumed.load_state_dict({**state, "conv_block.0.dropout_layer.nonsense": state["conv_first.bias"]})
+
+
 # ---------------------------------------------------------------- hardware only ----------------------------------------------------------------
 @pytest.mark.gpu
 def test_captured_training_step_draws_new_masks_at_every_replay():
