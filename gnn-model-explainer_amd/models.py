@@ -34,16 +34,17 @@ class LayerNorm(nn.Module):
             return ops.layer_norm(x, self.weight, self.bias, self.eps, relu=True)
         return F.layer_norm(F.relu(x), (self.dim,), self.weight, self.bias, self.eps)
 
-    def with_dropout(self, x, drop, use=None):
-        """(self(x), drop(self(x), use)) in one pass each way (ops.layer_norm_dropout)."""
-        return ops.layer_norm_dropout(x, self.weight, self.bias, drop.p, drop.seed, drop.step(use), self.eps, relu=True)
+    def with_dropout(self, x, drop, use=None, row_offset=0):
+        """(self(x), drop(self(x), use, row_offset)) in one pass each way (ops.layer_norm_dropout)."""
+        return ops.layer_norm_dropout(x, self.weight, self.bias, drop.p, drop.seed, drop.step(use), self.eps, relu=True, row_offset=row_offset)
 
 
 class CounterDropout(nn.Module):
     """Dropout whose mask is a function of (seed, use, layer, row, feature): ops.dropout.  `use` is the caller's number of this forward pass; left out, `uses` counts the
-    calls in training mode on the host and is part of the state_dict: a training run that is resumed goes on with the masks that come next.  A forward pass that is run again must draw the masks it drew first, which a count of calls cannot know: inside a backward pass
-    (recomputation, torch.utils.checkpoint) the use has to be given.  A step captured into a graph repeats the use it was captured with (ops.dropout takes a seed
-    tensor for new masks at every replay)."""
+    calls in training mode on the host and is part of the state_dict: a training run that is resumed goes on with the masks that come next.  A forward pass that is run
+    again must draw the masks it drew first, which a count of calls cannot know: inside a backward pass (recomputation, torch.utils.checkpoint) the use has to be given.
+    row_offset: where x's rows begin in the whole of which they are a shard.  A step captured into a graph repeats the use it was captured with (ops.dropout takes a
+    seed tensor for new masks at every replay)."""
 
     def __init__(self, p, seed, layer, layers):
         super().__init__()
@@ -69,8 +70,8 @@ class CounterDropout(nn.Module):
             self.uses = int(uses)
         super()._load_from_state_dict(state_dict, prefix, *rest)
 
-    def forward(self, x, use=None):
-        return ops.dropout(x, self.p, self.seed, self.step(use)) if self.training else x
+    def forward(self, x, use=None, row_offset=0):
+        return ops.dropout(x, self.p, self.seed, self.step(use), row_offset) if self.training else x
 
 
 class GraphConv(nn.Module):
@@ -167,13 +168,13 @@ class GcnEncoderGraph(nn.Module):
             if isinstance(m, CounterDropout):
                 m.uses = 0
 
-    def _activate(self, layer, x, nxt, use):
+    def _activate(self, layer, x, nxt, use, row_offset):
         """What follows graph convolution `layer` (models.py:239-253): (the layer's embedding, what convolution `nxt` reads, whether that has been through its
         dropout)."""
         drop = nxt.counter_dropout()
         if self.norms is not None:
             if drop is not None:
-                h, d = self.norms[layer].with_dropout(x, drop, use)
+                h, d = self.norms[layer].with_dropout(x, drop, use, row_offset)
                 return h, d, True
             x = self.norms[layer](x)
             return x, x, False
@@ -181,10 +182,10 @@ class GcnEncoderGraph(nn.Module):
         if self.bn:
             x = self.apply_bn(x)
         if drop is not None:
-            return x, drop(x, use), True
+            return x, drop(x, use, row_offset), True
         return x, x, False
 
-    def _layers(self, x, adj, dropout_use=None):
+    def _layers(self, x, adj, dropout_use=None, first_graph=0):
         """The graph convolutions one after the other: (embedding, attention adjacency) of each."""
         convs = [self.conv_first, *self.conv_block, self.conv_last]
         dropped = False
@@ -193,22 +194,23 @@ class GcnEncoderGraph(nn.Module):
             if i + 1 == len(convs):
                 yield x, adj_att
                 return
-            h, x, dropped = self._activate(i, x, convs[i + 1], dropout_use)
+            h, x, dropped = self._activate(i, x, convs[i + 1], dropout_use, first_graph * adj.shape[-1])
             yield h, adj_att
 
-    def gcn_forward(self, x, adj, dropout_use=None):
+    def gcn_forward(self, x, adj, dropout_use=None, first_graph=0):
         """models.py:230-267: all layers, concatenated embeddings [1, n, H (L - 1) + O] and the stacked attention adjacencies (the
         block layers re-append conv_first's, as the reference does at :252)."""
         x_all, att_all = [], []
-        for i, (h, adj_att) in enumerate(self._layers(x, adj, dropout_use)):
+        for i, (h, adj_att) in enumerate(self._layers(x, adj, dropout_use, first_graph)):
             x_all.append(h)
             att_all.append(att_all[0] if 0 < i <= len(self.conv_block) else adj_att)
         return torch.cat(x_all, dim=2), torch.stack(att_all, dim=3)
 
-    def forward(self, x, adj, batch_num_nodes=None, dropout_use=None, **kwargs):
-        """models.py:269-316: per-layer max over all rows, concat, linear head.  dropout_use: CounterDropout's use."""
+    def forward(self, x, adj, batch_num_nodes=None, dropout_use=None, first_graph=0, **kwargs):
+        """models.py:269-316: per-layer max over all rows, concat, linear head.  dropout_use: CounterDropout's use;
+        first_graph: the first graph's number in the whole batch of which this is a rank's share (its rows are counted from there)."""
         outs, atts = [], []
-        for h, adj_att in self._layers(x, adj, dropout_use):
+        for h, adj_att in self._layers(x, adj, dropout_use, first_graph):
             outs.append(h.max(dim=1)[0])
             atts.append(adj_att)
         output = torch.cat(outs, dim=1) if self.concat else outs[-1]
@@ -216,7 +218,8 @@ class GcnEncoderGraph(nn.Module):
 
 
 class GcnEncoderNode(GcnEncoderGraph):
-    def forward(self, x, adj, batch_num_nodes=None, dropout_use=None, **kwargs):
-        """models.py:363-376: the head on every row.  dropout_use: CounterDropout's use."""
-        emb, adj_att = self.gcn_forward(x, adj, dropout_use)
+    def forward(self, x, adj, batch_num_nodes=None, dropout_use=None, first_graph=0, **kwargs):
+        """models.py:363-376: the head on every row.  dropout_use: CounterDropout's use;
+        first_graph: the first graph's number in the whole batch of which this is a rank's share (its rows are counted from there)."""
+        emb, adj_att = self.gcn_forward(x, adj, dropout_use, first_graph)
         return self.pred_model(emb), adj_att

@@ -688,6 +688,28 @@ def test_a_resumed_training_run_goes_on_with_the_next_masks(be, tmp_path):
         resumed.load_state_dict({**state, "conv_block.0.dropout_layer.nonsense": state["conv_first.bias"]})
 
 
+@pytest.mark.parametrize("layer_norm", [False, True])
+@pytest.mark.parametrize("graph_mode", [False, True])
+def test_shares_of_a_batch_draw_the_whole_batches_masks(be, graph_mode, layer_norm):
+    """Data-parallel ranks: first_graph counts a share's rows from where it lies in the batch."""
+    g = torch.Generator().manual_seed(2)
+    adj, x = (torch.rand(5, 9, 9, generator=g) < 0.5).float().to(be.device), torch.randn(5, 9, 7, generator=g).to(be.device)
+    args = argparse.Namespace(method="base", bias=True, layer_norm=layer_norm, dropout_seed=9)
+    torch.manual_seed(3)
+    m = (models.GcnEncoderGraph if graph_mode else models.GcnEncoderNode)(7, 20, 20, 3, 4, bn=False, dropout=0.4, args=args).to(be.device).train()
+    with torch.no_grad():
+        whole = m(x, adj, dropout_use=3)[0]
+        # each graph's outputs are those of its own rows; the products over a smaller batch may add up in another order: the bound of the encoder against 64 bits above
+        at = 0
+        for share in (2, 1, 2):
+            part = m(x[at:at + share], adj[at:at + share], dropout_use=3, first_graph=at)[0]
+            assert torch.allclose(part, whole[at:at + share], rtol=0, atol=2e-4), at
+            if at:
+                same = m(x[at:at + share], adj[at:at + share], dropout_use=3)[0]      # the first share's masks: far beyond any rounding
+                assert (same - whole[at:at + share]).abs().max() > 1e-2
+            at += share
+
+
 # ---------------------------------------------------------------- hardware only ----------------------------------------------------------------
 @pytest.mark.gpu
 def test_captured_training_step_draws_new_masks_at_every_replay():
