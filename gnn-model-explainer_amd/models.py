@@ -52,6 +52,9 @@ class CounterDropout(nn.Module):
 
     def step(self, use=None):
         """The generator's step of the given use, or of the next one."""
+        if getattr(self, "_is_replica", False):
+            raise RuntimeError("seeded dropout in a replica of torch.nn.DataParallel: every replica would draw the same masks, and their count of uses is thrown away "
+                               "with them; run one process per GPU, each with its first_graph=")
         if use is None:
             if torch._C._current_graph_task_id() != -1:
                 raise RuntimeError("dropout drawn by a count of its calls, inside a backward pass: a recomputed forward pass would draw other masks than the first one; "

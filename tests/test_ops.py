@@ -710,6 +710,25 @@ def test_shares_of_a_batch_draw_the_whole_batches_masks(be, graph_mode, layer_no
             at += share
 
 
+def test_seeded_dropout_in_a_replica_of_data_parallel_is_refused(be):
+    """(_replicate_for_data_parallel is what torch.nn.DataParallel makes its copies with: no second device needed)"""
+    m = _encoder(models.GcnEncoderNode).to(be.device).train()
+    def replica(mod):
+        r = mod._replicate_for_data_parallel()
+        for k, v in mod._parameters.items():
+            setattr(r, k, v)
+        for k, v in mod._modules.items():
+            r._modules[k] = None if v is None else replica(v)
+        return r
+    r = replica(m)
+    x, adj = torch.randn(1, 6, 7, device=be.device), torch.ones(1, 6, 6, device=be.device)
+    for kw in ({}, {"dropout_use": 1}):
+        with pytest.raises(RuntimeError, match="DataParallel"):
+            r(x, adj, **kw)
+    m(x, adj)
+    assert torch.isfinite(replica(m.eval())(x, adj)[0]).all()
+
+
 # ---------------------------------------------------------------- hardware only ----------------------------------------------------------------
 @pytest.mark.gpu
 def test_captured_training_step_draws_new_masks_at_every_replay():
