@@ -133,12 +133,12 @@ Tensor like(const char* name, const py::object& o, const Tensor& x, at::IntArray
     return t;
 }
 
-int64_t integer(const char* name, const py::object& o, int64_t below) {
+int64_t integer(const char* name, const py::object& o, int64_t most) {
     const py::object n = py::reinterpret_steal<py::object>(PyNumber_Index(o.ptr()));
     if (!n) throw py::error_already_set();
     int over = 0;
     const long long v = PyLong_AsLongLongAndOverflow(n.ptr(), &over);
-    if (over || v < 0 || v >= below) throw py::value_error(text(name, " must be in [0, ", below, "), got ", std::string(py::str(n))));
+    if (over || v < 0 || v > most) throw py::value_error(text(name, " must be in [0, ", most, "], got ", std::string(py::str(n))));
     return v;
 }
 
@@ -154,8 +154,8 @@ Drop drop_of(const Tensor& x, double p, const py::object& seed, const py::object
     Drop d;
     if (!(p >= 0.0 && p <= 1.0)) throw py::value_error(text("p must be in [0, 1], got ", p));
     d.c.p = p;
-    d.c.step = (uint32_t)integer("step", step, int64_t(1) << 32);
-    d.c.row_offset = integer("row_offset", row_offset, int64_t(1) << 62);
+    d.c.step = (uint32_t)integer("step", step, UINT32_MAX);
+    d.c.row_offset = integer("row_offset", row_offset, (int64_t(1) << 62) - 1);
     if (THPVariable_Check(seed.ptr())) {
         d.state = THPVariable_Unpack(seed.ptr());
         if (d.state.scalar_type() != at::kLong || d.state.dim() != 1 || d.state.size(0) != 2 || !d.state.is_contiguous() || d.state.device() != x.device())

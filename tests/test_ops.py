@@ -429,6 +429,19 @@ def test_refusals(be):
             ops.dropout(x, 0.5, state)
 
 
+def test_the_ends_of_the_ranges_of_seed_step_and_row_offset(be):
+    """The largest of each, as a number and (seed, step) as a tensor: the masks of the definition; one more is refused."""
+    x = torch.randn(3, 11, generator=torch.Generator().manual_seed(1)).to(be.device)
+    for seed, step, row0 in (((1 << 63) - 1, 0, 0), ((1 << 63) - 1, (1 << 32) - 1, (1 << 62) - 1), (0, 0, 0)):
+        y = ops.dropout(x, 0.5, seed, step, row0)
+        keep = keep_mask(0.5, seed, step, np.arange(row0, row0 + 3, dtype=np.uint64), 11)
+        assert torch.equal(y.cpu(), torch.where(keep, 2 * x.cpu(), torch.zeros(())))
+        assert torch.equal(ops.dropout(x, 0.5, torch.tensor([seed, step], device=be.device), 0, row0), y)
+    for kw in (dict(seed=1 << 63), dict(seed=1, step=1 << 32), dict(seed=1, row_offset=1 << 62)):
+        with pytest.raises(ValueError, match="must be in"):
+            ops.dropout(x, 0.5, **kw)
+
+
 def test_forward_mode_derivatives_and_batched_tensors_are_refused(be):
     import torch.autograd.forward_ad as fwd
     x, w = torch.randn(4, 8, device=be.device), torch.ones(8, device=be.device)
