@@ -93,12 +93,30 @@ int type_of(const Tensor& x) {
     }
 }
 
+[[noreturn]] void not_implemented(const std::string& what) {
+    if (PyGILState_Check()) {
+        PyErr_SetString(PyExc_NotImplementedError, what.c_str());
+        throw py::error_already_set();
+    }
+    C10_THROW_ERROR(NotImplementedError, what);      // (a thread of the autograd engine)
+}
+
 // forward-mode derivatives would be lost without a word
 void no_tangent(const char* name, const Tensor& t) {
-    if (!t._fw_grad(/*level=*/0).defined()) return;
-    PyErr_SetString(PyExc_NotImplementedError, text(name, " carries a forward-mode derivative, which the operators do not propagate").c_str());
-    throw py::error_already_set();
+    if (t._fw_grad(/*level=*/0).defined()) not_implemented(text(name, " carries a forward-mode derivative, which the operators do not propagate"));
 }
+
+// A tensor that stands for others or for a computation (torch.func's batched and differentiated tensors, fake and functional ones, wrapper subclasses), or a sparse one,
+// has no memory of its own on its device; its null pointer would be read as an argument that is not there.
+bool has_memory(const Tensor& t) {
+    const c10::TensorImpl* impl = t.unsafeGetTensorImpl();
+    return !impl->key_set().has(c10::DispatchKey::Functionalize) && impl->has_storage() && impl->storage().device() == t.device();
+}
+void needs_memory(const char* name, const Tensor& t) {
+    if (!has_memory(t)) not_implemented(text(name, " is a tensor without memory of its own (sparse, batched, fake, functional or wrapped), which the operators cannot read"));
+}
+// ... nor has torch's zero tensor, whose elements are known without it.
+Tensor materialized(const Tensor& t) { return t.defined() && t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t; }
 
 Tensor input(const char* name, const py::object& o) {
     if (!THPVariable_Check(o.ptr()) || type_of(THPVariable_Unpack(o.ptr())) < 0)
@@ -107,7 +125,8 @@ Tensor input(const char* name, const py::object& o) {
     const Tensor& x = THPVariable_Unpack(o.ptr());
     if (x.dim() < 1) throw py::value_error(text(name, " needs at least one dimension"));
     if (g_lib.host ? !x.is_cpu() : !x.is_cuda()) throw std::runtime_error(text("the operators run on MI355X only (no CPU fallback): got a tensor on ", x.device()));
-    if (x.layout() != at::kStrided) throw py::type_error(text(name, " must be a dense tensor"));
+    if (x.layout() != at::kStrided || x.is_nested()) throw py::type_error(text(name, " must be a dense tensor"));
+    needs_memory(name, x);
     no_tangent(name, x);
     return x;
 }
@@ -120,6 +139,7 @@ Tensor parameter(const char* name, const py::object& o, const Tensor& x) {
         throw py::type_error(text(name, " must be float32 or of x's type ", x.scalar_type(), ", got ", p.scalar_type()));
     if (p.dim() != 1 || p.size(0) != x.size(-1)) throw py::value_error(text(name, " must have shape (", x.size(-1), ",), got ", p.sizes()));
     if (p.device() != x.device()) throw py::value_error(text(name, " is on ", p.device(), ", x on ", x.device()));
+    needs_memory(name, p);
     no_tangent(name, p);
     return p;
 }
@@ -130,6 +150,7 @@ Tensor like(const char* name, const py::object& o, const Tensor& x, at::IntArray
     const Tensor& t = THPVariable_Unpack(o.ptr());
     if (t.sizes() != shape || t.scalar_type() != type || t.device() != x.device())
         throw py::value_error(text(name, " must be ", shape, " ", type, " on ", x.device(), ", got ", t.sizes(), " ", t.scalar_type(), " on ", t.device()));
+    needs_memory(name, t);
     return t;
 }
 
@@ -161,6 +182,8 @@ Drop drop_of(const Tensor& x, double p, const py::object& seed, const py::object
         if (d.state.scalar_type() != at::kLong || d.state.dim() != 1 || d.state.size(0) != 2 || !d.state.is_contiguous() || d.state.device() != x.device())
             throw py::value_error(text("a seed tensor must be two contiguous int64 (seed, step) on x's device ", x.device(), ", got ", d.state.sizes(), " ",
                                        d.state.scalar_type(), " on ", d.state.device()));
+        needs_memory("a seed tensor", d.state);
+        d.state = materialized(d.state);
     } else {
         d.c.seed = (uint64_t)integer("seed", seed, INT64_MAX);
     }
@@ -173,9 +196,10 @@ struct Rows {
     int64_t rows = 0, cols = 0, stride = 0;
     const void* data() const { return t.defined() ? t.const_data_ptr() : nullptr; }
 };
-Rows rows_of(const Tensor& x) {
+Rows rows_of(const Tensor& given) {
     Rows m;
-    if (!x.defined()) return m;
+    if (!given.defined()) return m;
+    const Tensor x = materialized(given);
     m.cols = x.size(-1);
     m.rows = m.cols ? x.numel() / m.cols : 0;
     m.stride = m.cols;
@@ -215,11 +239,11 @@ struct NormCall {
         n.x_stride = x.stride;
         n.x = x.data();
         if (weight.defined()) {
-            w = weight.contiguous();
+            w = materialized(weight).contiguous();
             n.w = w.const_data_ptr();
         }
         if (bias.defined()) {
-            b = bias.contiguous();
+            b = materialized(bias).contiguous();
             n.b = b.const_data_ptr();
         }
         n.relu = relu;
@@ -301,6 +325,8 @@ struct NormNode : torch::autograd::Node {
         std::lock_guard<std::mutex> lock(mutex_);
         const Tensor dy = grads[0], dd = dropped ? grads[1] : Tensor();
         if (!dy.defined() && !dd.defined()) return variable_list(3);
+        for (const Tensor& g : {dy, dd})
+            if (g.defined()) needs_memory("a gradient", g);
         const Tensor xs = x.unpack(), ws = w.unpack();
         Drop d;
         d.c = drop;
@@ -323,6 +349,7 @@ struct DropoutNode : torch::autograd::Node {
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return variable_list(1);
+        needs_memory("a gradient", grads[0]);
         Drop d;
         d.c = drop;
         d.state = seed.unpack();
@@ -432,7 +459,7 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> backward_of(const py::object& 
     if (!g.defined() && !e.defined()) throw py::value_error(d ? "dh and dd are both None" : "dy is None");
     if (mean.is_none() || rstd.is_none()) throw py::value_error("mean and rstd must be given");
     const auto lead = i.x.sizes().slice(0, i.x.dim() - 1);
-    const Tensor m = like("mean", mean, i.x, lead, at::kFloat).contiguous(), r = like("rstd", rstd, i.x, lead, at::kFloat).contiguous();
+    const Tensor m = materialized(like("mean", mean, i.x, lead, at::kFloat)).contiguous(), r = materialized(like("rstd", rstd, i.x, lead, at::kFloat)).contiguous();
     const bool params = i.w.defined();
     NormGrads out = norm_backward(g, e, i.x, m.const_data_ptr<float>(), r.const_data_ptr<float>(), i.w, relu, d, params, params, params ? i.w.scalar_type() : at::kFloat);
     return {maybe(out.dx), maybe(out.dw), maybe(out.db)};

@@ -455,6 +455,35 @@ def test_forward_mode_derivatives_and_batched_tensors_are_refused(be):
         torch.func.grad(lambda v: ops.layer_norm(v, w).sum())(x)
 
 
+def test_tensors_without_memory_are_refused_or_materialised(be):
+    """What has no memory of its own must not be read as an argument that is not there (a weight of ones, the seed 0): torch's zero tensor counts as the zeros it is,
+    everything else is refused by name."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    x = torch.randn(4, 8, generator=torch.Generator().manual_seed(1)).to(be.device)
+    w, state = torch.rand(8, device=be.device) + 0.5, torch.tensor([0, 0], device=be.device)
+    y, mean, rstd = ops.layer_norm_forward(x, w)
+    zero = lambda *s, **kw: torch._efficientzerotensor(s, device=be.device, **kw)
+    assert torch.equal(ops.layer_norm(x, zero(8), w), ops.layer_norm(x, torch.zeros_like(w), w)) and torch.equal(ops.layer_norm(x, w, zero(8)), y)
+    assert torch.equal(ops.layer_norm(zero(4, 8), w, w), w.expand(4, 8)) and bool((ops.dropout(zero(4, 8), 0.5, 1) == 0).all())
+    assert torch.equal(ops.dropout(x, 0.5, zero(2, dtype=torch.int64)), ops.dropout(x, 0.5, 0))
+    for got, want in zip(ops.layer_norm_backward(zero(4, 8), x, zero(4), rstd, w), ops.layer_norm_backward(torch.zeros_like(x), x, torch.zeros_like(mean), rstd, w)):
+        assert torch.equal(got, want)
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        fx, fw, fs, fm = (mode.from_tensor(t) for t in (x, w, state, mean))
+    leaf = x.clone().requires_grad_()
+    for call in (lambda: ops.layer_norm(fx), lambda: ops.layer_norm(x, fw), lambda: ops.layer_norm(x, None, fw), lambda: ops.dropout(fx, 0.5, 1), lambda: ops.dropout(x, 0.5, fs),
+                 lambda: ops.layer_norm_backward(fx, x, mean, rstd), lambda: ops.layer_norm_backward(x, x, fm, rstd), lambda: ops.layer_norm(x, w.to_sparse()),
+                 lambda: ops.layer_norm_backward(x.to_sparse(), x, mean, rstd), lambda: torch.func.functionalize(ops.layer_norm)(x),
+                 lambda: torch.func.vmap(ops.layer_norm)(x), lambda: torch.func.vmap(lambda v: ops.layer_norm(x, v))(w.expand(3, 8)),
+                 lambda: torch.func.vmap(lambda s: ops.dropout(x, 0.5, s))(state.expand(3, 2)), lambda: torch.func.grad(lambda v: ops.layer_norm(v).sum())(x),
+                 lambda: torch.autograd.grad(ops.layer_norm(leaf), leaf, x.expand(3, 4, 8), is_grads_batched=True),
+                 lambda: torch.autograd.grad(ops.dropout(leaf, 0.5, 1), leaf, x.expand(3, 4, 8), is_grads_batched=True)):
+        with pytest.raises(NotImplementedError, match="without memory"):
+            call()
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        ops.layer_norm(torch.zeros(2, 2, dtype=torch.complex64, device=be.device))
+
+
 def test_tensors_off_the_gpu_are_refused():
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ops.dropout(torch.ones(2, 2), 0.5, 1)
