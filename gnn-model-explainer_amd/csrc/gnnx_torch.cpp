@@ -115,8 +115,8 @@ bool has_memory(const Tensor& t) {
 void needs_memory(const char* name, const Tensor& t) {
     if (!has_memory(t)) not_implemented(text(name, " is a tensor without memory of its own (sparse, batched, fake, functional or wrapped), which the operators cannot read"));
 }
-// ... nor has torch's zero tensor, whose elements are known without it.
-Tensor materialized(const Tensor& t) { return t.defined() && t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t; }
+// ... nor has torch's zero tensor, whose elements are known without it; and a view like the imaginary part of a conjugate has its elements' signs elsewhere.
+Tensor materialized(const Tensor& t) { return !t.defined() ? t : t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t.resolve_neg(); }
 
 Tensor input(const char* name, const py::object& o) {
     if (!THPVariable_Check(o.ptr()) || type_of(THPVariable_Unpack(o.ptr())) < 0)

@@ -484,6 +484,26 @@ def test_tensors_without_memory_are_refused_or_materialised(be):
         ops.layer_norm(torch.zeros(2, 2, dtype=torch.complex64, device=be.device))
 
 
+def test_views_of_the_opposite_sign(be):
+    """The imaginary part of a conjugate is a view of memory that holds its elements' negatives: one column of it is evenly spaced rows, read in place."""
+    g = torch.Generator().manual_seed(4)
+    z = torch.complex(torch.randn(5, 3, generator=g), torch.randn(5, 3, generator=g)).to(be.device).conj()
+    v, one = z.imag, torch.complex(torch.zeros(1), torch.tensor([2.0])).to(be.device).conj().imag      # one: [-2]
+    assert v.is_neg() and one.is_neg()
+    column = torch.tensor([[3.0], [4.0]], device=be.device)
+    for t in (v, v[:, 1:2], v[:, 1]):
+        plain = t.resolve_neg().clone()
+        assert torch.equal(ops.dropout(t, 0.5, 3), ops.dropout(plain, 0.5, 3)) and torch.equal(ops.layer_norm(t, relu=True), ops.layer_norm(plain, relu=True))
+        y, mean, rstd = ops.layer_norm_forward(plain)
+        assert torch.equal(ops.layer_norm_backward(t, plain, mean, rstd)[0], ops.layer_norm_backward(plain, plain, mean, rstd)[0])
+        leaf = plain.clone().requires_grad_()
+        assert torch.equal(torch.autograd.grad(ops.dropout(leaf, 0.5, 3), leaf, t)[0], ops.dropout(plain, 0.5, 3))
+    assert torch.equal(ops.layer_norm(column, None, one), torch.full_like(column, -2.0))       # (a row of one element is its mean)
+    y, mean, rstd = ops.layer_norm_forward(column)
+    assert torch.equal(ops.layer_norm_backward(column, column, one.expand(2), rstd, one.resolve_neg())[1],
+                       ops.layer_norm_backward(column, column, one.resolve_neg().expand(2).contiguous(), rstd, one)[1])
+
+
 def test_tensors_off_the_gpu_are_refused():
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ops.dropout(torch.ones(2, 2), 0.5, 1)
