@@ -151,6 +151,7 @@ Tensor like(const char* name, const py::object& o, const Tensor& x, at::IntArray
     if (t.sizes() != shape || t.scalar_type() != type || t.device() != x.device())
         throw py::value_error(text(name, " must be ", shape, " ", type, " on ", x.device(), ", got ", t.sizes(), " ", t.scalar_type(), " on ", t.device()));
     needs_memory(name, t);
+    no_tangent(name, t);
     return t;
 }
 
@@ -326,7 +327,10 @@ struct NormNode : torch::autograd::Node {
         const Tensor dy = grads[0], dd = dropped ? grads[1] : Tensor();
         if (!dy.defined() && !dd.defined()) return variable_list(3);
         for (const Tensor& g : {dy, dd})
-            if (g.defined()) needs_memory("a gradient", g);
+            if (g.defined()) {
+                needs_memory("a gradient", g);
+                no_tangent("a gradient", g);
+            }
         const Tensor xs = x.unpack(), ws = w.unpack();
         Drop d;
         d.c = drop;
@@ -350,6 +354,7 @@ struct DropoutNode : torch::autograd::Node {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return variable_list(1);
         needs_memory("a gradient", grads[0]);
+        no_tangent("a gradient", grads[0]);
         Drop d;
         d.c = drop;
         d.state = seed.unpack();

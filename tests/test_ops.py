@@ -504,6 +504,21 @@ def test_views_of_the_opposite_sign(be):
                        ops.layer_norm_backward(column, column, one.resolve_neg().expand(2).contiguous(), rstd, one)[1])
 
 
+def test_gradients_and_statistics_with_forward_mode_derivatives_are_refused(be):
+    import torch.autograd.forward_ad as fwd
+    x, w = torch.randn(4, 8, device=be.device), torch.ones(8, device=be.device)
+    y, mean, rstd = ops.layer_norm_forward(x, w)
+    leaf = x.clone().requires_grad_()
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ops.layer_norm_backward(dual(y), x, mean, rstd, w), lambda: ops.layer_norm_backward(y, x, dual(mean), rstd, w),
+                     lambda: ops.layer_norm_backward(y, x, mean, dual(rstd), w), lambda: ops.layer_norm_dropout_backward(y, dual(y), x, mean, rstd, w, 0.5, 1),
+                     lambda: torch.autograd.grad(ops.layer_norm(leaf, w), leaf, dual(y)), lambda: torch.autograd.grad(ops.dropout(leaf, 0.5, 1), leaf, dual(y)),
+                     lambda: torch.autograd.grad(ops.layer_norm_dropout(leaf, w, w, 0.5, 1)[1], leaf, dual(y))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+
+
 def test_tensors_off_the_gpu_are_refused():
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ops.dropout(torch.ones(2, 2), 0.5, 1)
