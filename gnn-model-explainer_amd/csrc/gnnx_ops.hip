@@ -3,7 +3,9 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 #include <limits>
 
 #include "../../include/gnnx.h"
@@ -43,6 +45,17 @@ const char* drop_args(const gnnx_drop* d, DropArgs* out) {
     out->row0 = d->row_offset;
     return nullptr;
 }
+
+// Whether an output (contiguous rows) shares memory with a matrix whose rows are `stride` elements apart.  It must not: two lanes may hold one element (a row's last
+// piece is moved back into the row, lanes beyond the last row repeat it) and one may read it after the other has stored it.
+bool overlap(const void* out, const void* in, int64_t stride, int64_t rows, int64_t cols, int32_t type) {
+    if (!out || !in || rows <= 0 || cols <= 0) return false;
+    const __int128 size = type == GNNX_F32 ? 4 : 2, row = cols * size, step = stride * size, lo = (__int128)(uintptr_t)out - (__int128)(uintptr_t)in, hi = lo + rows * row;
+    if (step == 0) return lo < row && hi > 0;
+    const __int128 r = lo < row ? 0 : (lo - row) / step + 1;      // the first row of `in` that ends behind the start of `out`
+    return r < rows && r * step < hi && r * step + row > lo;
+}
+const char* const OVERLAP = "an output shares memory with an input or with the other output";
 
 const char* norm_args(const gnnx_norm* n, NormArgs* a) {
     if (!n) return "null argument";
@@ -224,6 +237,9 @@ extern "C" int gnnx_layer_norm_forward(const gnnx_norm* n, const gnnx_drop* drop
     if ((a.d != nullptr) != (drop != nullptr)) return set_error("layer norm: a dropped output and its dropout go together");
     if ((a.mean != nullptr) != (a.rstd != nullptr)) return set_error("layer norm: mean and rstd go together");
     if (!a.x) return set_error("null argument");
+    for (const void* out : {a.y, a.d})
+        if (overlap(out, a.x, a.x_stride, a.rows, a.cols, n->type)) return set_error(OVERLAP);
+    if (overlap(a.y, a.d, a.cols, a.rows, a.cols, n->type)) return set_error(OVERLAP);
     const RowShape sh = forward_shape(n->type, a.cols);
     if (sh.lanes == LONG) {
         if (!workspace || workspace_bytes < workspace_bytes_of(n->type, a.rows, a.cols, false)) return set_error("workspace too small");
@@ -243,6 +259,9 @@ extern "C" int gnnx_layer_norm_backward(const gnnx_norm* n, const gnnx_drop* dro
     if (const char* e = drop_args(drop, &a.drop)) return set_error(e);
     if (a.rows > 0 && (a.dd != nullptr) != (drop != nullptr)) return set_error("layer norm: the gradient of a dropped output and its dropout go together");
     if (a.rows > 0 && ((!a.dy && !a.dd) || !a.x || !a.mean || !a.rstd || !a.dx)) return set_error("null argument");
+    if (overlap(a.dx, a.x, a.x_stride, a.rows, a.cols, n->type) || overlap(a.dx, a.dy, a.dy_stride, a.rows, a.cols, n->type) ||
+        overlap(a.dx, a.dd, a.dd_stride, a.rows, a.cols, n->type))
+        return set_error(OVERLAP);
     const RowShape sh = backward_shape(n->type, a.cols);
     const size_t needed = workspace_bytes_of(n->type, a.rows, a.cols, true);
     if ((a.dw || a.db || sh.lanes == LONG) && (!workspace || workspace_bytes < needed)) return set_error("workspace too small");
@@ -279,6 +298,7 @@ extern "C" int gnnx_dropout(int32_t type, int64_t rows, int64_t cols, const void
     if (rows < 0 || cols < 0 || x_stride < 0 || cols >= (int64_t(1) << 30)) return set_error("dropout: needs rows, stride >= 0 and 0 <= cols < 2^30");
     if (rows == 0 || cols == 0) return 0;
     if (!x || !y) return set_error("null argument");
+    if (overlap(y, x, x_stride, rows, cols, type)) return set_error(OVERLAP);
     a.rows = rows;
     a.cols = cols;
     a.stride = x_stride;

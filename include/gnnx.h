@@ -416,7 +416,7 @@ int gnnx_xl_run(gnnx_xl_handle h, const gnnx_hyper* hyper, const gnnx_xl_state* 
 /* ---- operators of an encoder's layers (csrc/gnnx_norm.hpp, csrc/gnnx_ops.hip) ----
  * What stands between two graph convolutions of an encoder (models.py:58-61, 230-267): layer norm with the ReLU before it, dropout, and the two in one pass,
  * each with its backward pass.  Matrices of `rows` rows and `cols` columns: the elements of a row contiguous, the rows of an INPUT its stride apart
- * (in elements; 0: every row the same), outputs contiguous; DEVICE pointers, aligned to their element; asynchronous on `stream`, which belongs to the current
+ * (in elements; 0: every row the same), outputs contiguous and apart from every input (a call in place is refused); DEVICE pointers, aligned to their element; asynchronous on `stream`, which belongs to the current
  * device.  Nothing is kept between calls, no call synchronises, allocates or clears memory through the runtime: all of them can be captured into a graph. */
 #define GNNX_F32 0
 #define GNNX_BF16 1

@@ -555,6 +555,44 @@ def test_the_c_entry_points_refuse_what_they_cannot_do(be):
     assert bool((out == 3.0).all())
 
 
+def test_the_c_entry_points_refuse_outputs_that_share_memory_with_inputs(be):
+    """(in place a row's last piece, moved back into the row, could read what another lane has stored; outputs in the gaps between an input's rows are apart from it)"""
+    lib = be.lib or engine.get_library()
+    rows, cols, pad = 6, 5, 40
+    base = torch.randn(rows, cols + pad, generator=torch.Generator().manual_seed(9)).to(be.device)
+    other, stats = torch.zeros(2, rows * cols, device=be.device), torch.ones(2, rows, device=be.device)
+    at = lambda r, c: base.data_ptr() + 4 * (r * (cols + pad) + c)
+    drop = engine._Drop(0.5, 1, None, 0, 0)
+    def dropout(y, x=at(0, 0), stride=cols + pad, r=rows):
+        return lib.gnnx_dropout(0, r, cols, x, stride, y, drop, None)
+    def forward(y, d=None):
+        n = engine._Norm(type=0, w_is_f32=1, rows=rows, cols=cols, x_stride=cols + pad, x=at(0, 0), y=y, d=d, eps=1e-5)
+        return lib.gnnx_layer_norm_forward(n, drop if d else None, None, 0, None)
+    def backward(dx, **kw):
+        n = engine._Norm(type=0, w_is_f32=1, rows=rows, cols=cols, x_stride=cols + pad, dy_stride=cols, dd_stride=cols, x=at(0, 0), dy=other[1].data_ptr(), dx=dx,
+                         mean=stats[0].data_ptr(), rstd=stats[1].data_ptr())
+        for k, v in kw.items():
+            setattr(n, k, v)
+        return lib.gnnx_layer_norm_backward(n, drop if n.dd else None, None, 0, None)
+    before, out = base.clone(), other[0].data_ptr()
+    inside = [at(0, 0), at(0, cols - 1), at(0, cols + 11), at(rows - 1, cols - 1), at(0, 0) - 4, at(2, 3), at(rows - 1, 0) - 4 * rows * cols + 4]
+    for y in inside:
+        for rc in (dropout(y), forward(y), forward(out, y), forward(y, out), backward(y)):
+            assert rc != 0 and b"shares memory" in lib.gnnx_last_error()
+    assert forward(out, out) != 0 and forward(out, out + 4) != 0
+    assert backward(other[1].data_ptr()) != 0 and backward(out, dd=out) != 0 and backward(out, dd=out + 4 * (rows * cols - 1)) != 0
+    assert dropout(at(0, 1), stride=0) != 0 and dropout(at(0, 0), stride=cols) != 0
+    assert torch.equal(base, before) and bool((other == 0).all())
+    # apart: behind the last row, before the first, between two rows that are one output apart
+    tail = torch.zeros(rows * cols, device=be.device)
+    assert dropout(tail.data_ptr()) == 0 and forward(tail.data_ptr()) == 0 and backward(tail.data_ptr()) == 0
+    want = ops.dropout(before[:4, :cols], 0.5, 1)
+    assert dropout(at(0, cols), r=4) == 0                                 # 20 elements in the gap of 40 behind the first row
+    if be.device != "cpu":
+        torch.cuda.synchronize()
+    assert torch.equal(base[0, cols:cols + 20].view(4, cols), want) and torch.equal(base[1:], before[1:])
+
+
 # ---------------------------------------------------------------- the encoders that call them ----------------------------------------------------------------
 def _encoder(cls, layers=4, p=0.4, **kw):
     torch.manual_seed(3)
