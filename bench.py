@@ -123,6 +123,15 @@ class Workload:
         return Subgraph(self.idx.sub_adjacency(nb), self.feat[nb], int(self.label[t]), int(row), np.argmax(self.pred[nb], 1), mask0)
 
 
+ORACLE_PROCESSES = 12
+
+
+def oracle_processes(sample):
+    """Worker processes of the CPU baseline.  Each opens the GPU although it computes on the CPU (torch's autograd engine asks for the device count at the first
+    backward pass, whatever devices are visible), and no more than 16 processes may hold one GPU here, this one among them."""
+    return max(1, min(sample, os.cpu_count() or 1, ORACLE_PROCESSES))
+
+
 def _oracle_worker(args):
     """One single-thread CPU process: the oracle ("port": torch-autograd restatement, bit-identical to the reference on
     CPU) on its share of the sample.  -> [(index, seconds, masked_adj, sigmoid(feat_mask))]"""
@@ -145,12 +154,12 @@ def _oracle_worker(args):
 
 def cpu_baselines(wl, sample, iters):
     """The oracle timed on this host's cores over a size-stratified sample of the same targets:
-      * process-parallel: one single-thread worker per sample target (the reference is dispatch-bound - ~700 tiny aten
+      * process-parallel: single-thread workers, oracle_processes of them (the reference is dispatch-bound - ~700 tiny aten
         ops per epoch - so one thread per target is its best configuration; 8 intra-op threads are slower);
       * one thread, one process, on a sub-sample.
     Returns (cpu_baseline dict, cpu_baseline_1thread dict, {sample index: (masked_adj, feat_sig)})."""
     import multiprocessing as mp
-    procs = max(1, min(len(sample), os.cpu_count() or 1))
+    procs = oracle_processes(len(sample))
     jobs = [([(k, s) for k, s in sample[p::procs]], wl.ck["sd"], iters) for p in range(procs)]
     ns = [s.adj.shape[0] for _, s in sample]
     t0 = time.perf_counter()
@@ -330,7 +339,7 @@ def bench_config4(args, dev, log):
         pick = order[np.linspace(0, G - 1, 32).astype(int)]
         sample = [(int(g), Subgraph(A[g], X[g], int(y[g]), 0, None, helpers.seeded_mask0(int(g), n).numpy())) for g in pick]
         import multiprocessing as mp
-        procs = max(1, min(len(sample), os.cpu_count() or 1))
+        procs = oracle_processes(len(sample))
         jobs = [([(k, sg) for k, sg in sample[p_::procs]], sd, args.iters, True) for p_ in range(procs)]
         with mp.get_context("spawn").Pool(procs) as pool:
             pool.map(_noop, range(procs))
