@@ -169,16 +169,16 @@ __device__ __forceinline__ Slot slot_at(uint32_t c, uint32_t cols) {      // col
 
 // The words of a piece's V elements from column c on (c is a multiple of 4 unless the piece was moved back from the end of a row that 4 does not divide: its words
 // then lie across V / 4 + 1 blocks).  They need nothing of the data: a kernel forms them while its loads are on their way, and compares them where it needs the
-// answer (truth values held that long are packed into bytes by the compiler, at 6 instructions each).
-template <class T>
-__device__ __forceinline__ void piece_words(const DropArgs& d, const DropKey& key, int64_t r, uint32_t c, uint32_t cols, uint32_t* out) {
+// answer (truth values of more than one piece held that long are packed into bytes by the compiler, at 6 instructions each).  put(j, word): takes the word of element j.
+template <class T, class Put>
+__device__ __forceinline__ void each_word(const DropArgs& d, const DropKey& key, int64_t r, uint32_t c, uint32_t cols, const Put& put) {
     constexpr int V = Piece<T>::V;
     if ((cols & 3) == 0) {
 #pragma unroll
         for (int h = 0; h < V; h += 4) {
             const Philox4 q = drop_words(d, key, r, (c >> 2) + h / 4);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) out[h + j] = q.w[j];
+            for (int j = 0; j < 4; ++j) put(h + j, q.w[j]);
         }
     } else {
         uint32_t w[V + 4];
@@ -193,9 +193,13 @@ __device__ __forceinline__ void piece_words(const DropArgs& d, const DropKey& ke
         for (int j = 0; j < V; ++j) {
             const uint32_t w0 = w[j], w1 = w[j + 1], w2 = w[j + 2], w3 = w[j + 3];      // (values: a choice between the elements would index memory)
             const uint32_t lo = sh & 1 ? w1 : w0, hi = sh & 1 ? w3 : w2;
-            out[j] = sh & 2 ? hi : lo;
+            put(j, sh & 2 ? hi : lo);
         }
     }
+}
+template <class T>
+__device__ __forceinline__ void piece_words(const DropArgs& d, const DropKey& key, int64_t r, uint32_t c, uint32_t cols, uint32_t* out) {
+    each_word<T>(d, key, r, c, cols, [out](int j, uint32_t word) { out[j] = word; });
 }
 
 // all ones in the bits of a piece's elements that count (all but the first `skip`)
@@ -350,18 +354,18 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a
         }
         uint32_t words[K][V];
         bool flags[V];
-        if (DROP)
+        if constexpr (DROP && K == 1) {
+            // one piece: lane masks in scalar registers, compared where the words are formed (65536 x 512 bf16 39.4 us, 256 columns 20.7; 41.0 and 21.6 where the
+            // words leave the generator's two branches first, 41.2 and 22.0 with words held)
+            each_word<T>(a.drop, key, r, at[0].c, (uint32_t)a.cols, [&](int j, uint32_t word) { flags[j] = kept(a.drop, word); });
+        } else if constexpr (DROP) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 piece_words<T>(a.drop, key, r, at[k].c, (uint32_t)a.cols, words[k]);
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    // one piece: lane masks in scalar registers (65536 x 512 bf16 43 us for 50 with words); more: the words - either way before the wait for the row,
-                    // which they move behind if left alone
-                    if constexpr (K == 1) flags[j] = kept(a.drop, words[k][j]);
-                    else GNNX_OPAQUE(words[k][j]);
-                }
+                for (int j = 0; j < V; ++j) GNNX_OPAQUE(words[k][j]);      // before the wait for the row: left alone they move behind the reductions
             }
+        }
         float s[1];
         if (full) s[0] = pieces_sum<true>(q, at, a.relu_floor);
         else s[0] = pieces_sum<false>(q, at, a.relu_floor);
