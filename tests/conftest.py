@@ -7,6 +7,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 if ROOT not in sys.path:
     sys.path.insert(0, ROOT)
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+os.environ.setdefault("GNNX_BUILD_STALE_ONLY", "1")      # __graft_entry__.build() from a test: the engine's unit takes minutes
 
 
 def pytest_configure(config):
