@@ -1,6 +1,6 @@
 """The encoder-layer operators (gnn_model_explainer_amd/ops.py): layer norm, counter-based dropout and the two in one pass, forward and backward, against their
-definitions in 64 bits, at the sizes where they can go wrong; their refusals; the encoders that call them.  Every case on two backends, the emulator build of the
-sources (CPU) and the HIP library (GPU).
+definitions in 64 bits, at the sizes where they can go wrong; their refusals; the encoders that call them.  On two backends: the HIP library (GPU) runs every case, the
+emulator build of the sources (CPU) the smaller ones, each in one type, with one of every launch shape among them.
 
 Tolerances are a priori.  u = 2^-24 is the relative error of one fp32 operation, h = finfo(type).eps / 2 that of the one rounding at the store (plus half of the
 type's smallest subnormal), L the longest chain of additions of a row sum, of which the kernels have at most cols / 64 + 16 (64 lanes or more share a row of more
@@ -184,6 +184,83 @@ def test_layer_norm_forward_and_backward_against_64_bits(on, name, rows, cols, d
         for g, (want, bound), what in zip(got, back, ("dx", "dw", "db")):
             if g is not None:
                 assert_close(g, want, bound, what)
+
+
+# one of every launch shape: each number of lanes and pieces per lane of the forward pass, the backward pass's workgroups of few and many waves and of two pieces per lane,
+# long rows in chunks (several rows per walk), more than 16 partial rows of dw and db
+LAUNCHES = [(3, 4, torch.float32), (5, 6, torch.float32), (3, 13, torch.float32), (3, 30, torch.float32), (2, 61, torch.float32), (2, 125, torch.float32),
+            (2, 250, torch.float32), (2, 511, torch.float32), (2, 767, torch.float32), (2, 1021, torch.float32), (2, 2047, torch.float32), (2, 3001, torch.float32),
+            (2, 4095, torch.float32), (2, 5000, torch.float32), (3, 8193, torch.float32), (700, 3, torch.float16), (1500, 9, torch.bfloat16), (2, 8193, torch.bfloat16),
+            (3, 16383, torch.bfloat16), (5, 16387, torch.float16)]
+
+
+@pytest.mark.parametrize("rows,cols,dtype", LAUNCHES)
+def test_every_launch_shape_on_the_emulator(on, rows, cols, dtype):
+    test_layer_norm_forward_and_backward_against_64_bits(on, "emu", rows, cols, dtype)
+    test_layer_norm_dropout_against_64_bits(on, "emu", rows, cols, dtype)
+    test_dropout_against_its_definition(on, "emu", rows, cols, dtype)
+
+
+def _whole_numbers(be, rows, cols, dtype, seed=0):
+    """x, dh, dd of small whole numbers on the device: with mean 0 and rstd 1 given (and p = 1/2, whose scale is 2) every product and every partial sum of dw and db is a
+    whole number below 2^24, exact in fp32 in whatever order."""
+    g = torch.Generator(device=be.device).manual_seed(1000 * rows + cols + seed)
+    assert rows * 3 * 9 < 1 << 24
+    return [torch.randint(-3, 4, (rows, cols), generator=g, device=be.device).to(dtype) for _ in range(3)]
+
+
+MANY = [(40000, 3), (300000, 3), (300000, 7), (40000, 20), (99997, 20), (99997, 60), (20000, 130), (20000, 513), (5000, 4095), (3000, 8190), (700, 16385), (200, 65537)]
+
+
+def _many_cases():
+    out = [pytest.param("emu", r, c, t, id="emu-%dx%d-%s" % (r, c, str(t)[6:]))
+           for r, c, t in ((4000, 3, torch.float32), (3000, 7, torch.bfloat16), (1500, 9, torch.bfloat16), (1100, 20, torch.float32), (90, 513, torch.float16),
+                           (9, 5000, torch.float32), (9, 8193, torch.bfloat16))]
+    return out + [pytest.param("gpu", r, c, t, id="gpu-%dx%d-%s" % (r, c, str(t)[6:]), marks=pytest.mark.gpu) for r, c in MANY for t in TYPES]
+
+
+@pytest.mark.parametrize("name,rows,cols,dtype", _many_cases())
+def test_no_row_is_lost_or_counted_twice_in_the_parameters_gradients(on, name, rows, cols, dtype):
+    """dw and db, exact: one row more or less, in any lane's or workgroup's share, shows."""
+    be = on(name)
+    x, dh, dd = _whole_numbers(be, rows, cols, dtype)
+    mean, rstd, w = torch.zeros(rows, device=be.device), torch.ones(rows, device=be.device), torch.ones(cols, device=be.device)
+    sums = lambda dy: ((dy.double() * x.double()).sum(0), dy.double().sum(0))
+    _, dw, db = ops.layer_norm_backward(dh, x, mean, rstd, w)
+    for got, want in zip((dw, db), sums(dh)):
+        assert torch.equal(got.double(), want)
+    kept = ops.dropout(torch.ones_like(x), 0.5, 7, 3).double()            # 2 or 0: ops.dropout against its definition is a test of its own
+    _, dw, db = ops.layer_norm_dropout_backward(dh, dd, x, mean, rstd, w, 0.5, 7, 3)
+    for got, want in zip((dw, db), sums(dh.double() + dd.double() * kept)):
+        assert torch.equal(got.double(), want)
+    # one row alone
+    for r in {0, rows // 2, rows - 1}:
+        one = torch.zeros_like(dh)
+        one[r] = dh[r]
+        _, dw, db = ops.layer_norm_backward(one, x, mean, rstd, w)
+        assert torch.equal(dw, dh[r].float() * x[r].float()) and torch.equal(db, dh[r].float())
+
+
+@pytest.mark.parametrize("name,rows,cols,dtype", [c for c in _many_cases() if c.values[1] * c.values[2] < 1 << 24])
+def test_the_parameters_gradients_of_many_rows_against_64_bits(on, name, rows, cols, dtype):
+    """As above with ordinary numbers.  A column's longest chain of additions is a lane's walk over its share of the rows (at most rows / parts, the workgroups that leave a
+    partial row each), at most 6 + 4 additions across the lanes and waves of a workgroup, and the join of the partial rows: parts / 32 + 36 (or up to 16 one by one)."""
+    be = on(name)
+    lib = be.lib or engine.get_library()
+    x, dy, _, w, _ = make(be, rows, cols, dtype, torch.float32)
+    _, mean, rstd = ops.layer_norm_forward(x, w)
+    _, dw, db = ops.layer_norm_backward(dy, x, mean, rstd, w)
+    nbytes = lib.gnnx_layer_norm_workspace_bytes(TYPES.index(dtype), rows, cols, 1)
+    parts = nbytes // (8 * cols)                                          # (long rows keep a little more there: at least this many workgroups' share)
+    if cols > 8192:
+        parts = 1
+    chain = -(-rows // parts) + parts / 32 + 64
+    xd, dyd, md, rd = x.double(), dy.double(), mean.double()[:, None], rstd.double()[:, None]
+    xhat = (xd - md) * rd
+    # each term: xhat's two roundings, the product fused into the sum, and the chain's
+    for got, terms, each in ((dw, dyd * xhat, 3), (db, dyd, 0)):
+        want, size = terms.sum(0), terms.abs().sum(0)
+        assert got.dtype == torch.float32 and bool(((got.double() - want).abs() <= 1.01 * (chain + each) * U * size + 2.0 ** -149).all())
 
 
 @pytest.mark.parametrize("name,rows,cols,dtype", _cases())
