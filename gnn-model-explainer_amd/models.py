@@ -139,7 +139,7 @@ class GcnEncoderGraph(nn.Module):
         if args is not None and getattr(args, "layer_norm", False):
             if self.bn:
                 raise ValueError("bn and layer_norm are two normalisations of the same rows: choose one")
-            self.norms = nn.ModuleList([LayerNorm(hidden_dim) for _ in range(num_layers - 1)])
+            self.norms = nn.ModuleList([LayerNorm(hidden_dim) for _ in range(len(self.conv_block) + 1)])
         self.act = nn.ReLU()
         self.label_dim = label_dim
         self.pred_input_dim = hidden_dim * (num_layers - 1) + embedding_dim if concat else embedding_dim

@@ -766,6 +766,19 @@ def test_encoder_options_keep_what_was(monkeypatch):
         engine.model_arrays(m.state_dict())
 
 
+@pytest.mark.parametrize("layers", [1, 2])
+def test_encoders_without_a_middle_layer(be, layers):
+    """(an encoder always has its first and last convolution, whatever num_layers says; without concatenation it runs with num_layers = 1 too)"""
+    args = argparse.Namespace(method="base", bias=True, layer_norm=True, dropout_seed=9)
+    torch.manual_seed(3)
+    m = models.GcnEncoderGraph(7, 20, 20, 3, layers, concat=False, bn=False, dropout=0.4, args=args).to(be.device).train()
+    assert len(m.norms) == 1
+    x, adj = torch.randn(2, 6, 7, device=be.device), torch.ones(2, 6, 6, device=be.device)
+    out, _ = m(x, adj)
+    h = m.norms[0](m.conv_first(x, adj)[0])
+    assert torch.equal(out, m.pred_model(m.conv_last(h, adj)[0].max(dim=1)[0]))
+
+
 def test_explanations_with_seeded_dropout_are_reproducible(be, tmp_path, monkeypatch):
     """An encoder with layer norm and seeded dropout through Explainer.explain (the PyTorch-ROCm route, dropout active as in the reference: explain.py:135): a target's
     explanation does not depend on what was explained before it nor on torch's generators."""
