@@ -110,20 +110,24 @@ def explain_one(model, sub_adj, sub_feat, sub_label, pred_label, node_idx_new, a
     sched, opt = make_optimizer(args, params)
     model.eval()
     mod.train()                      # explain.py:135: this flips the wrapped model to train mode too (dropout)
-    if hasattr(model, "reset_dropout"):      # counter-based dropout: the same masks for this target whatever was explained before it
-        model.reset_dropout()
+    # counter-based dropout: the same masks for this target whatever was explained before it; a training run's own count goes on afterwards
+    uses = model.reset_dropout() if hasattr(model, "reset_dropout") else None
     adj_atts = None
-    for _ in range(int(args.num_epochs)):
-        mod.zero_grad()
-        opt.zero_grad()
-        ypred, adj_atts = mod(node_idx_new, unconstrained=unconstrained)
-        loss = mod.loss(ypred, pred_label, node_idx_new)
-        loss.backward()
-        opt.step()
-        if sched is not None:
-            sched.step()
-        if kind != "exp":            # explain.py:200-201: the attention baseline only needs one forward
-            break
+    try:
+        for _ in range(int(args.num_epochs)):
+            mod.zero_grad()
+            opt.zero_grad()
+            ypred, adj_atts = mod(node_idx_new, unconstrained=unconstrained)
+            loss = mod.loss(ypred, pred_label, node_idx_new)
+            loss.backward()
+            opt.step()
+            if sched is not None:
+                sched.step()
+            if kind != "exp":            # explain.py:200-201: the attention baseline only needs one forward
+                break
+    finally:
+        if uses:
+            model.reset_dropout(uses)
     model.train(was_training)
     sub = np.asarray(sub_adj, np.float64)
     if kind == "exp":

@@ -165,11 +165,14 @@ class GcnEncoderGraph(nn.Module):
         """models.py:222-228: a fresh BatchNorm1d(num_nodes) in training mode - every node standardised over its features."""
         return F.batch_norm(x, None, None, None, None, True, 0.1, 1e-5)
 
-    def reset_dropout(self):
-        """Every CounterDropout starts its uses again: what follows draws the masks that a new model would."""
-        for m in self.modules():
-            if isinstance(m, CounterDropout):
-                m.uses = 0
+    def reset_dropout(self, uses=None):
+        """Every CounterDropout starts its uses again: what follows draws the masks that a new model would.  Returns the counts so far, with which (as `uses`) another
+        call goes on where they were."""
+        drops = [m for m in self.modules() if isinstance(m, CounterDropout)]
+        before = [m.uses for m in drops]
+        for m, n in zip(drops, uses or [0] * len(drops)):
+            m.uses = n
+        return before
 
     def _activate(self, layer, x, nxt, use, row_offset):
         """What follows graph convolution `layer` (models.py:239-253): (the layer's embedding, what convolution `nxt` reads, whether that has been through its

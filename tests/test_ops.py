@@ -805,6 +805,29 @@ def test_explanations_with_seeded_dropout_are_reproducible(be, tmp_path, monkeyp
     assert np.isfinite(a).all() and np.array_equal(a, b) and (a != 0).any()
 
 
+def test_an_explanation_leaves_the_count_of_a_training_run_alone(be, tmp_path, monkeypatch):
+    import helpers
+    from gnn_model_explainer_amd.explainer import explain
+    from test_explainer_api import _args as api_args
+    monkeypatch.setitem(explain._ENGINE, "device", be.device)
+    ck = helpers.load_ckpt("syn1")
+    args = api_args(tmp_path, 3, "syn1", layer_norm=True, dropout_seed=7)
+    model = models.GcnEncoderNode(ck["feat"].shape[1], 20, 20, ck["pred"].shape[1], 4, bn=False, dropout=0.3, args=args).to(be.device).train()
+    x, adj = torch.randn(1, 5, ck["feat"].shape[1], device=be.device), torch.ones(1, 5, 5, device=be.device)
+    model(x, adj), model(x, adj)
+    ex = explain.Explainer(model, ck["adj"][None].astype(np.float64), ck["feat"][None].astype(np.float64), ck["label"][None], ck["pred"][None], None, args,
+                           writer=None, print_training=False, graph_mode=False, graph_idx=-1)
+    ex.explain(302)
+    assert [c.dropout_layer.uses for c in model.conv_block] == [2, 2]
+    def broken(e):
+        raise ArithmeticError("no head")
+    monkeypatch.setattr(model.pred_model, "forward", broken)
+    with pytest.raises(ArithmeticError):
+        ex.explain(302)
+    assert [c.dropout_layer.uses for c in model.conv_block] == [2, 2]
+    assert model.reset_dropout() == [2, 2] and model.reset_dropout([5, 5]) == [0, 0] and model.reset_dropout() == [5, 5]
+
+
 def test_command_line_run_of_such_an_encoder(be, tmp_path, monkeypatch):
     """The command line from a checkpoint of an encoder with layer norm: --layer-norm rebuilds it, --dropout and --dropout-seed act during the explanation, twice alike."""
     import helpers
