@@ -11,8 +11,8 @@
 #pragma once
 #include <stdint.h>
 
-// No contraction by the compiler: every fma below is written out, so the variants of a kernel (with or without dropout, with or without the parameters' gradients,
-// whatever the shape of the launch adds up first) round an element alike.
+// No contraction by the compiler: every fma below is written out, so the variants of one launch shape (with or without dropout, with or without the parameters'
+// gradients) round an element alike.  (Another launch shape, as rows cut into chunks, takes the row's sums in another order.)
 #pragma clang fp contract(off)
 
 namespace gnnx {
@@ -321,10 +321,10 @@ __device__ __forceinline__ float pieces_squares(const Piece<T> (&q)[K], const Sl
 }
 
 // The forward pass: one read of x, mean and then the squared distances from it out of the registers (no E[v^2] - mean^2), one write of each output.
-// Bound by HBM: 65536 x 1024 fp32 90 us = 5.98 TB/s, bf16 (fp32 parameters) 45 us = 5.96, 16384 x 4096 bf16 41 us = 6.6 - a copy reaches 6.1.  One row per group of
+// Bound by HBM: 65536 x 1024 fp32 90 us = 5.96 TB/s, bf16 (fp32 parameters) 46 us = 5.8, 16384 x 4096 bf16 41 us = 6.6 - a copy reaches 6.1.  One row per group of
 // lanes and no walk over rows: a grid that covers all rows at once streams better than workgroups that stride (copies: 6.1 against 4.4 to 5.6 TB/s).  With a second,
-// dropped output the generator's 40 instructions per four elements fill what the loads leave (65536 x 1024 bf16: 75 us, 93 % of the VALU's issue slots before the
-// words were compared in place, fp32 137 us = 5.9 TB/s).
+// dropped output the generator's 40 instructions per four elements fill what the loads leave (65536 x 1024 bf16: 74 us, the VALU busy 69 % of the time, 512 columns
+// 39 us and 75 %; fp32 137 us = 5.9 TB/s, 35 %).
 template <class T, class P, int TPR, int K, bool DROP>
 __global__ __launch_bounds__(norm_threads<TPR>()) void k_norm_forward(NormArgs a) {
     constexpr int V = Piece<T>::V, RPB = norm_threads<TPR>() / TPR;
@@ -402,7 +402,7 @@ __device__ __forceinline__ void chunk_slots(Slot (&at)[CHUNK_PIECES], int ch, in
 }
 
 // x is read twice (forward) and x, dy twice (backward), the second time from the caches where they hold it; a workgroup per row left most of the chip idle and read
-// the row three times (48 x 65537 fp32, both passes: 787 us; in chunks 32).  A long row's two statistics are 8 bytes per chunk.
+// the row three times (48 x 65537 fp32, both passes: 787 us; in chunks 30).  A long row's two statistics are 8 bytes per chunk.
 // First launch of the forward pass: the chunk's mean and its sum of squared distances from that mean.
 template <class T>
 __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_stats(NormArgs a) {
@@ -494,7 +494,7 @@ __global__ __launch_bounds__(CHUNK_LANES) void k_norm_chunk_outputs(NormArgs a) 
     }
 }
 
-// Rows shorter than one piece (fewer than 4 or 8 columns): one thread per row, element by element (10^6 x 7 bf16: 22 us = 1.3 TB/s, bound by the 2-byte accesses).
+// Rows shorter than one piece (fewer than 4 or 8 columns): one thread per row, element by element (10^6 x 7 bf16: 24 us = 1.2 TB/s, bound by the 2-byte accesses).
 template <class T, bool DROP>
 __global__ __launch_bounds__(256) void k_norm_forward_narrow(NormArgs a) {
     const float inv = 1.0f / (float)a.cols;
@@ -609,8 +609,8 @@ __device__ __forceinline__ void store_cols(const NormArgs& a, int64_t part, cons
 
 // The backward pass of rows in registers: one pass over x, dy (and dd), dx out.  COLS: a workgroup walks rows a grid apart and keeps its share of dw and db in
 // registers; at the end the lanes that hold the same column add up (lane sums, then LDS across the waves) and the workgroup leaves one partial row of each.
-// Bound by HBM at fp32 (65536 x 1024: 150 us = 5.4 TB/s of x, dy and dx), at 16 bits by HBM and 170 instructions per piece together (83 us = 4.8 TB/s, a 42 % busy
-// VALU, with 5 us of it the join of the partial rows).
+// Bound by HBM at fp32 (65536 x 1024: 145 us = 5.6 TB/s), at 16 bits by HBM and 164 instructions per piece together (80 us = 5.2 TB/s with the VALU busy 44 % of the
+// time; 5 us more are the join of the partial rows).
 // The next row is always on its way while one is worked on (the last one is loaded again at the end: a load that may or may not have been issued would make
 // the wait for the row before it a wait for everything).
 template <class T, class P, int TPR, int K, bool DROP, bool COLS>
@@ -928,8 +928,8 @@ struct DropoutArgs {
     DropArgs drop;
 };
 
-// One thread per piece of a row, the words formed before the load returns.  Bound by HBM: 16384 x 4096 bf16 41 us = 6.5 TB/s, 65536 x 1024 fp32 88 us = 6.1 (a copy:
-// 6.1); at 16 bits the generator's 10 instructions per element are close behind (63 % of the VALU's issue slots).  32 bits per element and 10 rounds cost nothing over
+// One thread per piece of a row, the words formed before the load returns.  Bound by HBM: 16384 x 4096 bf16 42 us = 6.4 TB/s, 65536 x 1024 fp32 87 us = 6.2 (a copy:
+// 6.1); at 16 bits the generator's 10 instructions per element are close behind (the VALU is busy 69 % of the time, 41 % at fp32).  32 bits per element and 10 rounds cost nothing over
 // 16 bits or 7 rounds there.  BIG: more pieces in all than 32 bits count.
 template <class T, bool BIG>
 __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {

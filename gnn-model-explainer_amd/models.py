@@ -21,7 +21,8 @@ from . import ops
 
 
 class LayerNorm(nn.Module):
-    """LayerNorm over the features of relu(x), one gain and offset per feature; on the GPU one kernel (ops.layer_norm), the ReLU in it."""
+    """LayerNorm over the features of relu(x), one gain and offset per feature; on the GPU one kernel (ops.layer_norm), the ReLU in it, for x in float32, bfloat16 or
+    float16 (other types are refused there)."""
 
     def __init__(self, dim, eps=1e-5):
         super().__init__()

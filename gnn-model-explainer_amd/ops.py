@@ -17,7 +17,8 @@ an int64 tensor (seed, step) on x's device that the kernel reads when it runs (`
 advances that tensor in the graph and draws a new mask at every replay.  row_offset: where x's first row lies in the tensor of which x is a shard.  A dropped
 element is 0 whatever it was.
 
-The calls run on the current stream of x's device and can be captured into graphs.  There is no CPU fallback: tensors elsewhere are refused.  Argument checks, outputs
+The calls run on the current stream of x's device and can be captured into graphs.  There is no CPU fallback: tensors elsewhere are refused, as are tensors without memory
+of their own (sparse, batched, fake, functional) and tensors that carry forward-mode derivatives.  Gradients cannot be differentiated again.  Argument checks, outputs
 and the autograd nodes are csrc/gnnx_torch.cpp (a call is a few microseconds of host time); the kernels and the C ABI below it are libgnnx_hip.so."""
 import importlib.machinery
 import importlib.util
